@@ -72,6 +72,7 @@ typedef struct har_cuda_weights har_cuda_weights;
 typedef struct har_cuda_moe_layer har_cuda_moe_layer;
 typedef struct har_cuda_ep har_cuda_ep;
 typedef struct har_cuda_gguf har_cuda_gguf;
+typedef struct har_cuda_i8_weights har_cuda_i8_weights;
 
 /* ---- context ------------------------------------------------------------
  * Replaces the device/queue pair HAR opens per model
@@ -159,6 +160,89 @@ int32_t har_cuda_q6k_gemv(har_cuda_ctx *ctx, const har_cuda_weights *w, int64_t 
  * 6-bit sub-block scales (offset 32), f16 d. */
 int32_t har_cuda_q3k_gemv(har_cuda_ctx *ctx, const har_cuda_weights *w, int64_t expert,
                           const float *x_dev, int64_t M, float *y_dev);
+
+/* ---- 8-bit integer products with scales per token and channel ----------------
+ * No reference counterpart: the dense product of many token rows (an LM head
+ * over a prompt, a projection) that the block-quantised GEMVs above leave out.
+ * Element types of float operands: */
+#define HAR_CUDA_DTYPE_F32 0
+#define HAR_CUDA_DTYPE_F16 1
+#define HAR_CUDA_DTYPE_BF16 2
+/* Rows to 8-bit integers: scale[m] = max_k |x[m][k]| / 127 and q[m][k] =
+ * x[m][k] / scale[m] rounded to the nearest integer (halves to even), both
+ * quotients rounded to f32 first; |q| <= 127.  A row of zeros has scale 0 and
+ * q 0; a row holding a NaN or an infinity has scale NaN and q 0, so every
+ * product with it is NaN.  x_dev [M][K] of `dtype`, rows ldx elements apart;
+ * q_dev [M][K], rows ldq bytes apart (bytes between K and ldq are left as they
+ * are); scale_dev f32 [M]. */
+int32_t har_cuda_i8_quantize(har_cuda_ctx *ctx, const void *x_dev, int32_t dtype, int64_t M,
+                             int64_t K, int64_t ldx, int8_t *q_dev, int64_t ldq,
+                             float *scale_dev);
+/* A weight matrix [N][K] in 8-bit integers with one scale per row (output
+ * channel).  quantize: the same rule over the rows of a float matrix; the
+ * handle owns its copy.  wrap: an existing device matrix, 16-byte aligned, rows
+ * ldq bytes apart (a multiple of 16; bytes between K and ldq are never used),
+ * not freed by the library.  Values of -128 are allowed; K <= 131,056, the
+ * longest sum that 32 bits hold. */
+int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32_t dtype,
+                                     int64_t N, int64_t K, int64_t ldw,
+                                     har_cuda_i8_weights **out);
+int32_t har_cuda_i8_weights_wrap(har_cuda_ctx *ctx, const int8_t *q_dev, int64_t ldq,
+                                 const float *scale_dev, int64_t N, int64_t K,
+                                 har_cuda_i8_weights **out);
+/* The caller makes sure that no work that reads the weights is in flight. */
+int32_t har_cuda_i8_weights_free(har_cuda_i8_weights *w);
+/* y[m][n] = f32(sum_k q[m][k] * w[n][k]) * f32(scale[m] * w_scale[n]), the
+ * integer sum exact, the product rounded to f32 and then to y's type.  q_dev
+ * [M][K] 16-byte aligned, rows ldq bytes apart (a multiple of 16), scale_dev
+ * f32 [M]; y_dev [M][N] of `y_dtype`, rows ldy elements apart. */
+int32_t har_cuda_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q_dev,
+                           int64_t ldq, const float *scale_dev, int64_t M, void *y_dev,
+                           int32_t y_dtype, int64_t ldy);
+/* The same from float rows: quantises x_dev [M][K] (rows ldx elements apart)
+ * and multiplies; bit for bit har_cuda_i8_quantize followed by
+ * har_cuda_i8_matmul.  The quantised rows live in workspace_dev (16-byte
+ * aligned, at least har_cuda_i8_linear_workspace(w, M) bytes), or with NULL in
+ * the context's scratch arena.  While the stream is being captured a call that
+ * needs workspace takes it from the caller only (HAR_CUDA_ERR_ARG with NULL): a
+ * graph must not keep an address that a later call may free. */
+int64_t har_cuda_i8_linear_workspace(const har_cuda_i8_weights *w, int64_t M);
+int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x_dev,
+                           int32_t x_dtype, int64_t ldx, int64_t M, void *y_dev, int32_t y_dtype,
+                           int64_t ldy, void *workspace_dev, size_t workspace_bytes);
+
+/* ---- log probabilities of given tokens, entropy, top alternatives ------------
+ * No reference counterpart (its serving step ends in logits,
+ * har/crates/har-serve/src/adapter.rs:74-113): what scoring a prompt and a
+ * completion's logprobs read from them.  For each row of logits_dev [T][V]
+ * (rows ldl elements apart), with M = max x and Z = sum exp(x - M) in f32:
+ *   logprobs[t][g] = (x[tokens[t][g]] - M) - log Z   (f32 [T][G]),
+ *   entropy[t]     = log Z - sum exp(x - M) (x - M) / Z, in nats (f32 [T]),
+ *   top_ids / top_logprobs [T][k]: the k largest logits, ties to the lower id.
+ * tokens_dev int32 [T][G]: -1 is padding and scores 0; any other id outside
+ * [0, V) scores NaN and sets the device error word (HAR_CUDA_ERR_DEVICE at the
+ * next har_cuda_synchronize).  A logit of -inf is a masked token; a row of
+ * nothing else has log probabilities -inf, entropy 0 and the ids 0, 1, ... on
+ * top.  A row holding a NaN or +inf has NaN in every float output (NaN counts
+ * as the lowest value for top_ids).  Entries past V alternatives are id -1,
+ * -inf.  0 <= k <= 32, 0 <= G; a null output (with G or k > 0, too) is not
+ * written, and tokens_dev may be null when G is 0 or logprobs_dev null. */
+#define HAR_CUDA_LOGPROBS_MAX_TOP 32
+int32_t har_cuda_token_logprobs(har_cuda_ctx *ctx, const void *logits_dev, int32_t dtype, int64_t T,
+                                int64_t V, int64_t ldl, const int32_t *tokens_dev, int32_t G,
+                                int32_t k, float *logprobs_dev, float *entropy_dev,
+                                int32_t *top_ids_dev, float *top_logprobs_dev);
+/* har_cuda_token_logprobs of the logits that har_cuda_i8_linear would write as
+ * f32 for the LM head w [V][K] and hidden states x_dev [T][K], without the
+ * [T][V] logits in memory.  Workspace as for har_cuda_i8_linear, of
+ * har_cuda_i8_head_workspace bytes. */
+int64_t har_cuda_i8_head_workspace(const har_cuda_i8_weights *w, int64_t T, int32_t G, int32_t k);
+int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *w,
+                                  const void *x_dev, int32_t x_dtype, int64_t ldx, int64_t T,
+                                  const int32_t *tokens_dev, int32_t G, int32_t k,
+                                  float *logprobs_dev, float *entropy_dev, int32_t *top_ids_dev,
+                                  float *top_logprobs_dev, void *workspace_dev,
+                                  size_t workspace_bytes);
 
 /* ---- router top-k ---------------------------------------------------------
  * Per token: softmax over all E logits with max subtraction, experts ordered

@@ -287,7 +287,7 @@ int32_t har_cuda_synchronize(har_cuda_ctx *ctx, int64_t timeout_ms) {
     cudaStreamSynchronize(ctx->stream);
     std::string why = "a kernel reported device error word " + std::to_string(word);
     if (word & DEV_ERR_TIMEOUT) why += " (a bounded wait ran out)";
-    if (word & DEV_ERR_BOUNDS) why += " (an expert id out of range)";
+    if (word & DEV_ERR_BOUNDS) why += " (an expert or token id out of range)";
     if (word & DEV_ERR_RANGE)
       why += " (a value beyond the tensor-core path's f16 range -- |x|, a sub-block sum or a SwiGLU "
              "output >= 65520 -- or an unrepresentable Q4_K block: run it with HAR_CUDA_MOE_FORCE_GEMV)";

@@ -1,0 +1,81 @@
+// score.cuh — shared by the 8-bit integer products and the log-probability
+// kernels: the weight handle, element types, the order of alternatives, and
+// the kernel launchers that score.cu's entry points call.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "har_internal.cuh"
+
+// A weight matrix [N][K] in 8-bit integers, one f32 scale per row.
+struct har_cuda_i8_weights {
+  const int8_t *q = nullptr;
+  const float *scale = nullptr;
+  int64_t N = 0, K = 0, ldq = 0;
+  int device = 0;
+  bool owned = false;  // q and scale share one allocation, at q
+};
+
+namespace har {
+
+// Longest row whose integer sum fits in 32 bits with every product at its
+// largest, 128 * 128: 131,071, rounded down to whole 16-byte pieces.
+constexpr int64_t I8_MAX_K = 131056;
+constexpr int I8_MAX_TOP = HAR_CUDA_LOGPROBS_MAX_TOP;
+
+inline size_t dtype_bytes(int32_t dtype) { return dtype == HAR_CUDA_DTYPE_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Order of alternatives as one unsigned 64-bit key: larger value first, then
+// lower index.  The high word orders floats (-0 and +0 alike, NaN below -inf);
+// the low word is the complement of the index.  0 is below every entry.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.0f));
+  if (v != v) return 0u;
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t o) {
+  if (o == 0u) return __int_as_float(0x7fffffff);
+  return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ unsigned long long order_key(float v, uint32_t id) {
+  return ((unsigned long long)order_bits(v) << 32) | (0xffffffffu - id);
+}
+
+// Calls f with a value of the element type that `dtype` names.
+template <typename F>
+auto with_dtype(int32_t dtype, F &&f) {
+  if (dtype == HAR_CUDA_DTYPE_F32) return f(float());
+  if (dtype == HAR_CUDA_DTYPE_F16) return f(__half());
+  return f(__nv_bfloat16());
+}
+
+// The outputs of one log-probability call; any of them may be null.
+struct LogprobOut {
+  const int32_t *tokens;
+  int G, k;
+  float *logprobs, *entropy, *top_logprobs;
+  int32_t *top_ids;
+  int *status;  // the context's device error word
+};
+
+int32_t launch_i8_quantize(har_cuda_ctx *ctx, const void *x, int32_t dtype, int64_t M, int64_t K,
+                           int64_t ldx, int8_t *q, int64_t ldq, float *scale);
+int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q,
+                         int64_t ldq, const float *scale, int64_t M, void *y, int32_t y_dtype,
+                         int64_t ldy);
+int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
+                              int64_t V, int64_t ldl, const LogprobOut &out);
+
+}  // namespace har

@@ -50,6 +50,10 @@ MOE_FORCE_TC = 0x8
 MOE_EMPTY_SLOTS = 0x10
 MOE_TC_F16W = 0x20
 MOE_DECODE = 0x40
+# element types of float operands (har_cuda.h: HAR_CUDA_DTYPE_*)
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+I8_MAX_K = 131056       # longest row of an 8-bit product: 32-bit sums stay exact
+LOGPROBS_MAX_TOP = 32   # alternatives a row can list
 
 # Every symbol include/har_cuda.h declares (tests check the library exports them).
 EXPORTS = [
@@ -74,6 +78,10 @@ EXPORTS = [
     "har_cuda_ep_exchange_mode",
     "har_cuda_slot_table_create", "har_cuda_slot_table_free", "har_cuda_slot_table_storage",
     "har_cuda_slot_table_last_error", "har_cuda_slot_reserve", "har_cuda_slot_mark_upload_submitted",
+    "har_cuda_i8_quantize", "har_cuda_i8_weights_quantize", "har_cuda_i8_weights_wrap",
+    "har_cuda_i8_weights_free", "har_cuda_i8_matmul", "har_cuda_i8_linear_workspace",
+    "har_cuda_i8_linear", "har_cuda_token_logprobs", "har_cuda_i8_head_workspace",
+    "har_cuda_i8_head_logprobs",
     "har_cuda_slot_upload", "har_cuda_slot_mark_ready", "har_cuda_slot_acquire",
     "har_cuda_slot_release", "har_cuda_slot_evict", "har_cuda_slot_table_snapshot",
 ]
@@ -186,6 +194,17 @@ def load_library() -> C.CDLL:
         "har_cuda_moe_stack": (i32, [vp, vp, i32, vp, i64, i32, vp, vp, vp, u32]),
         "har_cuda_gen_q4k": (i32, [vp, vp, i64, i64, u64, i64, C.c_float, C.c_float]),
         "har_cuda_moe_stack_host": (i32, [vp, vp, i32, vp, i64, i32, vp, vp, vp, u32]),
+        "har_cuda_i8_quantize": (i32, [vp, vp, i32, i64, i64, i64, vp, i64, vp]),
+        "har_cuda_i8_weights_quantize": (i32, [vp, vp, i32, i64, i64, i64, pp]),
+        "har_cuda_i8_weights_wrap": (i32, [vp, vp, i64, vp, i64, i64, pp]),
+        "har_cuda_i8_weights_free": (i32, [vp]),
+        "har_cuda_i8_matmul": (i32, [vp, vp, vp, i64, vp, i64, vp, i32, i64]),
+        "har_cuda_i8_linear_workspace": (i64, [vp, i64]),
+        "har_cuda_i8_linear": (i32, [vp, vp, vp, i32, i64, i64, vp, i32, i64, vp, C.c_size_t]),
+        "har_cuda_token_logprobs": (i32, [vp, vp, i32, i64, i64, i64, vp, i32, i32, vp, vp, vp, vp]),
+        "har_cuda_i8_head_workspace": (i64, [vp, i64, i32, i32]),
+        "har_cuda_i8_head_logprobs": (i32, [vp, vp, vp, i32, i64, i64, vp, i32, i32, vp, vp, vp, vp,
+                                            vp, C.c_size_t]),
         "har_cuda_profile_begin": (i32, [vp]),
         "har_cuda_moe_ffn_noalloc": (i32, [vp, vp, vp, i64, i32, vp, vp, vp, u32]),
         "har_cuda_profile_end": (i32, [vp, C.c_char_p, C.c_size_t, vp, i64, C.POINTER(C.c_int64)]),
@@ -218,6 +237,47 @@ def _dptr(t) -> int:
         raise HarCudaError(ERR_ARG, "expected a CUDA tensor")
     if not t.is_contiguous():
         raise HarCudaError(ERR_ARG, "expected a contiguous tensor")
+    return t.data_ptr()
+
+
+_dtype_ids = None
+
+
+def _dtype(t, what: str) -> int:
+    """HAR_CUDA_DTYPE_* of a float tensor."""
+    global _dtype_ids
+    if _dtype_ids is None:
+        import torch
+        _dtype_ids = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+    d = _dtype_ids.get(t.dtype)
+    if d is None:
+        raise HarCudaError(ERR_ARG, f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return d
+
+
+def _matrix(t, device: int, what: str):
+    """(rows, columns, device pointer, elements between rows) of a 2-D CUDA
+    tensor whose rows are contiguous (a slice of a wider one will do)."""
+    if not t.is_cuda or t.get_device() != device:
+        raise HarCudaError(ERR_ARG, f"{what}: expected a tensor on cuda:{device}")
+    if t.dim() != 2:
+        raise HarCudaError(ERR_GEOMETRY, f"{what}: expected a matrix, got {t.dim()} dimensions")
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if step != 1 and cols > 1:
+        raise HarCudaError(ERR_ARG, f"{what}: the elements of a row must be contiguous")
+    return rows, cols, t.data_ptr(), ld if rows > 1 else cols
+
+
+def _vector(t, device: int, dtype_name: str, shape, what: str):
+    """Device pointer of a contiguous tensor of this type and shape."""
+    if not t.is_cuda or t.get_device() != device:
+        raise HarCudaError(ERR_ARG, f"{what}: expected a tensor on cuda:{device}")
+    if str(t.dtype) != dtype_name:
+        raise HarCudaError(ERR_ARG, f"{what}: expected {dtype_name}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise HarCudaError(ERR_GEOMETRY, f"{what}: expected shape {shape}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise HarCudaError(ERR_ARG, f"{what}: expected a contiguous tensor")
     return t.data_ptr()
 
 
@@ -375,6 +435,121 @@ class Context:
         self.check(self.lib.har_cuda_q6k_gemv(self.handle, w.handle, expert, _dptr(x), M,
                                               _dptr(y)))
         return y
+
+    # ---- 8-bit integer products -----------------------------------------------
+    def i8_quantize(self, x, q, scale):
+        """Rows of x [M][K] (float32/float16/bfloat16) to 8-bit integers q [M][K]
+        with scale f32 [M]: scale = max|x| / 127, q = round(x / scale), halves to
+        even.  q's rows may be slices of wider ones; i8_matmul needs them to start
+        at multiples of 16 bytes (i8_rows makes such a matrix)."""
+        M, K, xp, ldx = _matrix(x, self.device, "i8_quantize: x")
+        Mq, Kq, qp, ldq = _matrix(q, self.device, "i8_quantize: q")
+        if (Mq, Kq) != (M, K):
+            raise HarCudaError(ERR_GEOMETRY, "i8_quantize: x and q differ in shape")
+        if str(q.dtype) != "torch.int8":
+            raise HarCudaError(ERR_ARG, f"i8_quantize: q must be int8, got {q.dtype}")
+        sp = _vector(scale, self.device, "torch.float32", (M,), "i8_quantize: scale")
+        self.check(self.lib.har_cuda_i8_quantize(self.handle, xp, _dtype(x, "i8_quantize: x"), M, K, ldx,
+                                                 qp, ldq, sp))
+        return q, scale
+
+    def i8_weights(self, w) -> "I8Weights":
+        """A float matrix [N][K] on the device as 8-bit integers with a scale
+        per row, in memory of the handle's own."""
+        N, K, wp, ldw = _matrix(w, self.device, "i8_weights")
+        h = C.c_void_p()
+        self.check(self.lib.har_cuda_i8_weights_quantize(self.handle, wp, _dtype(w, "i8_weights"), N, K,
+                                                         ldw, C.byref(h)))
+        return I8Weights(self, h, N, K)
+
+    def wrap_i8(self, q, scale) -> "I8Weights":
+        """An existing int8 matrix q [N][K] (rows at multiples of 16 bytes) and
+        its scales f32 [N] as weights; the tensors stay the caller's."""
+        N, K, qp, ldq = _matrix(q, self.device, "wrap_i8: q")
+        if str(q.dtype) != "torch.int8":
+            raise HarCudaError(ERR_ARG, f"wrap_i8: q must be int8, got {q.dtype}")
+        sp = _vector(scale, self.device, "torch.float32", (N,), "wrap_i8: scale")
+        h = C.c_void_p()
+        self.check(self.lib.har_cuda_i8_weights_wrap(self.handle, qp, ldq, sp, N, K, C.byref(h)))
+        w = I8Weights(self, h, N, K)
+        w.keepalive = (q, scale)
+        return w
+
+    def i8_matmul(self, w: "I8Weights", q, scale, y):
+        """y [M][N] = (q w^T) * scale * w.scale for rows quantised by
+        i8_quantize; y float32, float16 or bfloat16."""
+        M, K, qp, ldq = _matrix(q, self.device, "i8_matmul: q")
+        My, N, yp, ldy = _matrix(y, self.device, "i8_matmul: y")
+        if K != w.K or N != w.N or My != M:
+            raise HarCudaError(ERR_GEOMETRY, f"i8_matmul: q [M][{w.K}], y [M][{w.N}]")
+        if str(q.dtype) != "torch.int8":
+            raise HarCudaError(ERR_ARG, f"i8_matmul: q must be int8, got {q.dtype}")
+        sp = _vector(scale, self.device, "torch.float32", (M,), "i8_matmul: scale")
+        self.check(self.lib.har_cuda_i8_matmul(self.handle, w.handle, qp, ldq, sp, M, yp,
+                                               _dtype(y, "i8_matmul: y"), ldy))
+        return y
+
+    def _workspace(self, t, what: str):
+        if t is None:
+            return None, 0
+        if not t.is_cuda or t.get_device() != self.device or not t.is_contiguous():
+            raise HarCudaError(ERR_ARG, f"{what}: the workspace must be contiguous on cuda:{self.device}")
+        return t.data_ptr(), t.numel() * t.element_size()
+
+    def i8_linear(self, w: "I8Weights", x, y, workspace=None):
+        """y [M][N] = x w^T through 8 bits: x [M][K] quantised per row, then
+        i8_matmul.  workspace: a device tensor of w.linear_workspace(M) bytes,
+        needed only while a CUDA graph is captured; else the context's arena."""
+        M, K, xp, ldx = _matrix(x, self.device, "i8_linear: x")
+        My, N, yp, ldy = _matrix(y, self.device, "i8_linear: y")
+        if K != w.K or N != w.N or My != M:
+            raise HarCudaError(ERR_GEOMETRY, f"i8_linear: x [M][{w.K}], y [M][{w.N}]")
+        wp, wb = self._workspace(workspace, "i8_linear")
+        self.check(self.lib.har_cuda_i8_linear(self.handle, w.handle, xp, _dtype(x, "i8_linear: x"), ldx, M,
+                                               yp, _dtype(y, "i8_linear: y"), ldy, wp, wb))
+        return y
+
+    # ---- log probabilities -----------------------------------------------------
+    def _logprob_args(self, T: int, tokens, logprobs, entropy, top_ids, top_logprobs, what: str):
+        """(tokens, G, k, outputs) of a log-probability call; outputs may be None."""
+        dev = self.device
+        G = 0 if tokens is None else tokens.shape[1] if tokens.dim() == 2 else -1
+        k = top_ids.shape[-1] if top_ids is not None else top_logprobs.shape[-1] if top_logprobs is not None else 0
+        tp = None if tokens is None else _vector(tokens, dev, "torch.int32", (T, G), f"{what}: tokens")
+        if logprobs is not None and tokens is None:
+            raise HarCudaError(ERR_ARG, f"{what}: log probabilities need tokens")
+        lp = None if logprobs is None else _vector(logprobs, dev, "torch.float32", (T, G), f"{what}: logprobs")
+        ep = None if entropy is None else _vector(entropy, dev, "torch.float32", (T,), f"{what}: entropy")
+        ip = None if top_ids is None else _vector(top_ids, dev, "torch.int32", (T, k), f"{what}: top_ids")
+        bp = None if top_logprobs is None else _vector(top_logprobs, dev, "torch.float32", (T, k),
+                                                       f"{what}: top_logprobs")
+        return tp, G, k, lp, ep, ip, bp
+
+    def token_logprobs(self, logits, tokens=None, logprobs=None, entropy=None, top_ids=None,
+                       top_logprobs=None):
+        """For each row of logits [T][V] (float32/float16/bfloat16): log
+        probabilities f32 [T][G] of the given tokens int32 [T][G] (-1: padding,
+        scores 0), entropy f32 [T] in nats, and the k largest alternatives, ids
+        int32 [T][k] (ties to the lower id) with log probabilities f32 [T][k].
+        Outputs that are None are not computed.  -inf masks a token."""
+        T, V, xp, ldl = _matrix(logits, self.device, "token_logprobs: logits")
+        self.check(self.lib.har_cuda_token_logprobs(
+            self.handle, xp, _dtype(logits, "token_logprobs: logits"), T, V, ldl,
+            *self._logprob_args(T, tokens, logprobs, entropy, top_ids, top_logprobs, "token_logprobs")))
+
+    def i8_head_logprobs(self, w: "I8Weights", x, tokens=None, logprobs=None, entropy=None, top_ids=None,
+                         top_logprobs=None, workspace=None):
+        """token_logprobs of the logits x w^T (as i8_linear writes them in f32)
+        for hidden states x [T][K] and an LM head w [V][K], without the logits
+        in memory.  workspace as for i8_linear, of w.head_workspace(T, G, k) bytes."""
+        T, K, xp, ldx = _matrix(x, self.device, "i8_head_logprobs: x")
+        if K != w.K:
+            raise HarCudaError(ERR_GEOMETRY, f"i8_head_logprobs: x [T][{w.K}]")
+        wp, wb = self._workspace(workspace, "i8_head_logprobs")
+        self.check(self.lib.har_cuda_i8_head_logprobs(
+            self.handle, w.handle, xp, _dtype(x, "i8_head_logprobs: x"), ldx, T,
+            *self._logprob_args(T, tokens, logprobs, entropy, top_ids, top_logprobs, "i8_head_logprobs"),
+            wp, wb))
 
     def route_topk(self, logits, k: int, ids, weights):
         T, E = logits.shape
@@ -628,6 +803,44 @@ class Q4KWeights:
             self.free()
         except Exception:
             pass
+
+
+class I8Weights:
+    """A device matrix [N][K] in 8-bit integers with one f32 scale per row."""
+
+    def __init__(self, ctx: Context, handle, N: int, K: int):
+        self.ctx, self.handle, self.N, self.K = ctx, handle, N, K
+        self.keepalive = None
+
+    @property
+    def nbytes(self) -> int:
+        return self.N * (self.K + 4)
+
+    def linear_workspace(self, M: int) -> int:
+        """Bytes of workspace that i8_linear takes for M rows (0: none)."""
+        return int(self.ctx.lib.har_cuda_i8_linear_workspace(self.handle, M))
+
+    def head_workspace(self, T: int, G: int, k: int) -> int:
+        """Bytes of workspace that i8_head_logprobs takes."""
+        return int(self.ctx.lib.har_cuda_i8_head_workspace(self.handle, T, G, k))
+
+    def free(self):
+        if self.handle:
+            self.ctx.lib.har_cuda_i8_weights_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def i8_rows(M: int, K: int, device):
+    """An empty int8 matrix [M][K] whose rows start at multiples of 16 bytes, as
+    i8_matmul and wrap_i8 take them."""
+    import torch
+    return torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :K]
 
 
 class Gguf:

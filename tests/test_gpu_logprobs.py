@@ -1,0 +1,280 @@
+"""Log probabilities of given tokens, entropy and top alternatives against the
+definition in 64 bits, from logits and straight from hidden states."""
+import math
+
+import pytest
+import torch
+
+import har_cuda
+from score_util import check_logprobs, logprobs64, product, quantize64
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = har_cuda.Context(0)
+    yield c
+    c.close()
+
+
+def outputs(T, G, k):
+    f = dict(dtype=torch.float32, device="cuda")
+    return {"logprobs": torch.full((T, G), 5.0, **f), "entropy": torch.full((T,), 5.0, **f),
+            "ids": torch.full((T, k), 5, dtype=torch.int32, device="cuda"), "top": torch.full((T, k), 5.0, **f)}
+
+
+def score(ctx, logits, tokens, k):
+    o = outputs(logits.shape[0], tokens.shape[1], k)
+    ctx.token_logprobs(logits, tokens, o["logprobs"], o["entropy"], o["ids"], o["top"])
+    ctx.synchronize()
+    return o
+
+
+def given(seed, T, V, G):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(0, V, (T, G), generator=g, dtype=torch.int32).cuda()
+
+
+def logits_of(seed, T, V, dtype, pad=0, std=2.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, V + pad, generator=g) * std).to(DT[dtype]).cuda()[:, :V]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T,V,G,k,pad", [(1, 1, 1, 1, 0), (1, 2, 2, 5, 0), (3, 31, 1, 32, 1), (2, 33, 0, 3, 0),
+                                         (5, 257, 3, 20, 2), (1, 1000, 1, 0, 0), (4, 4099, 1, 20, 0),
+                                         (1, 50021, 1, 20, 0), (2, 50021, 2, 32, 3), (160, 700, 1, 5, 1),
+                                         (400, 1203, 1, 2, 0), (1, 131072, 1, 20, 0), (3, 131072, 1, 1, 8),
+                                         (40, 16384, 1, 8, 0)])
+def test_rows(ctx, dtype, T, V, G, k, pad):
+    x = logits_of(T + V + k, T, V, dtype, pad)
+    tok = given(V, T, V, G)
+    check_logprobs(score(ctx, x, tok, k), logprobs64(x, tok, k), (dtype, T, V))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [40, 5000, 70001])
+def test_masks_and_values_that_are_not_numbers(ctx, dtype, V):
+    """-inf masks; a row of nothing else; one token left; the type's lowest
+    value; +inf and NaN; ties between far apart ids; an outlier; +0 and -0."""
+    x = logits_of(V, 11, V, dtype)
+    low = torch.finfo(DT[dtype]).min
+    x[0, 1:] = -math.inf
+    x[1] = -math.inf
+    x[2] = -math.inf
+    x[2, V - 1] = 3.0
+    x[3] = low
+    x[4, V // 2:] = low
+    x[5, 7] = math.inf
+    x[6, V - 2] = math.nan
+    x[7] = 1.5
+    x[8] = 0.0
+    x[8, ::2] = -0.0
+    x[9, 5] = 60000.0
+    x[10, ::3] = -math.inf
+    tok = torch.stack([torch.arange(11) % V, torch.full((11,), V - 1), torch.full((11,), -1)], 1).int().cuda()
+    check_logprobs(score(ctx, x, tok, 20), logprobs64(x, tok, 20), (dtype, V))
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_orders_that_insert_every_value(ctx, T):
+    """Ascending and descending rows, few distinct values: the candidate lists
+    turn over as often as they can."""
+    V = 9001
+    up = torch.arange(V, dtype=torch.float32) * 1e-3
+    x = torch.stack([up, up.flip(0), (torch.arange(V) % 3).float(), torch.where(torch.arange(V) > V - 30, 1.0, 0.0)])
+    x = x.repeat((T + 3) // 4, 1)[:T].cuda()
+    tok = given(1, T, V, 1)
+    n = min(T, 8)
+    got = score(ctx, x, tok, 32)
+    ref = logprobs64(x[:n], tok[:n], 32)
+    check_logprobs({k: v[:n] for k, v in got.items()}, ref, T)
+    for i in range(n, T):
+        assert torch.equal(got["ids"][i], got["ids"][i % 4]) and torch.equal(got["top"][i], got["top"][i % 4])
+
+
+def test_tokens_outside_the_vocabulary(ctx):
+    x = logits_of(3, 2, 100, "f32")
+    for bad in (100, -2, 2 ** 31 - 1, -2 ** 31):
+        tok = torch.tensor([[4, -1], [bad, 7]], dtype=torch.int32, device="cuda")
+        o = outputs(2, 2, 3)
+        ctx.token_logprobs(x, tok, o["logprobs"], o["entropy"], o["ids"], o["top"])
+        with pytest.raises(har_cuda.HarCudaError) as e:
+            ctx.synchronize()
+        assert e.value.status == har_cuda.ERR_DEVICE
+        check_logprobs(o, logprobs64(x, tok, 3))
+    ctx.synchronize()                          # the error word was read and cleared
+
+
+def test_outputs_left_out(ctx):
+    x, tok = logits_of(4, 6, 999, "bf16"), given(4, 6, 999, 2)
+    full = score(ctx, x, tok, 5)
+    for keep in ("logprobs", "entropy", "ids", "top"):
+        o = outputs(6, 2, 5)
+        a = {n: (v if n == keep else None) for n, v in o.items()}
+        ctx.token_logprobs(x, tok if keep == "logprobs" else None, a["logprobs"], a["entropy"], a["ids"], a["top"])
+        assert torch.equal(o[keep], full[keep]), keep
+    ctx.token_logprobs(x)                      # nothing asked for
+
+
+def test_no_rows_and_repeated_rows(ctx):
+    o = outputs(0, 1, 2)
+    ctx.token_logprobs(torch.empty(0, 9, device="cuda"), torch.empty(0, 1, dtype=torch.int32, device="cuda"),
+                       o["logprobs"], o["entropy"], o["ids"], o["top"])
+    x = logits_of(5, 1, 777, "f16")
+    tok = given(6, 7, 777, 1)
+    ref = logprobs64(x.expand(7, 777), tok, 4)
+    check_logprobs(score(ctx, x.expand(7, 777), tok, 4), ref)
+
+
+def test_results_do_not_change_from_call_to_call(ctx):
+    x, tok = logits_of(8, 3, 40000, "f32"), given(9, 3, 40000, 1)
+    a = score(ctx, x, tok, 20)
+    for _ in range(5):
+        b = score(ctx, x, tok, 20)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_refusals(ctx):
+    x, tok = logits_of(10, 4, 50, "f32"), given(11, 4, 50, 2)
+    o = outputs(4, 2, 3)
+
+    def refused(status, *a, **k):
+        with pytest.raises(har_cuda.HarCudaError) as e:
+            ctx.token_logprobs(*a, **k)
+        assert e.value.status == status, e.value
+
+    refused(har_cuda.ERR_ARG, x.double(), tok, o["logprobs"])
+    refused(har_cuda.ERR_ARG, x.cpu(), tok, o["logprobs"])
+    refused(har_cuda.ERR_ARG, x, tok.long(), o["logprobs"])
+    refused(har_cuda.ERR_ARG, x, None, o["logprobs"])
+    refused(har_cuda.ERR_GEOMETRY, x, tok[:3], o["logprobs"])
+    refused(har_cuda.ERR_GEOMETRY, x, tok, o["logprobs"][:, :1])
+    refused(har_cuda.ERR_GEOMETRY, x, tok, o["logprobs"], o["entropy"][:3])
+    refused(har_cuda.ERR_GEOMETRY, x, None, None, None, o["ids"], o["top"][:, :2])
+    refused(har_cuda.ERR_GEOMETRY, x, None, None, None, torch.empty(4, 33, dtype=torch.int32, device="cuda"))
+    refused(har_cuda.ERR_GEOMETRY, x[0], tok, o["logprobs"])
+    refused(har_cuda.ERR_ARG, x.t().contiguous().t(), tok, o["logprobs"])
+    refused(har_cuda.ERR_GEOMETRY, torch.empty(4, 0, device="cuda"), None, None, o["entropy"])
+
+
+# ---- from hidden states -----------------------------------------------------------------
+
+
+def head_of(ctx, seed, V, K):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-127, 128, (V, (K + 15) // 16 * 16), generator=g, dtype=torch.int8).cuda()[:, :K]
+    s = ((torch.rand(V, generator=g) + 0.5) * 2.5 / (73 * math.sqrt(K))).cuda()
+    return ctx.wrap_i8(q, s), q, s
+
+
+def head_score(ctx, w, x, tok, k, **kw):
+    o = outputs(x.shape[0], tok.shape[1], k)
+    ctx.i8_head_logprobs(w, x, tok, o["logprobs"], o["entropy"], o["ids"], o["top"], **kw)
+    return o
+
+
+@pytest.mark.parametrize("T,V,K,G,k,dtype", [(1, 1, 16, 1, 1, "f32"), (1, 300, 64, 1, 20, "f32"), (2, 33, 17, 2, 32, "f16"),
+                                             (3, 2000, 256, 1, 5, "bf16"), (8, 5003, 2048, 1, 20, "f32"),
+                                             (17, 1025, 100, 0, 3, "f32"), (40, 3001, 333, 3, 0, "bf16"),
+                                             (130, 1500, 128, 1, 5, "f32"), (203, 2777, 199, 2, 32, "f16"),
+                                             (300, 513, 512, 1, 1, "f32"), (129, 9000, 64, 1, 20, "f32")])
+def test_head(ctx, T, V, K, G, k, dtype):
+    """The logits are those of i8_linear bit for bit, so alternatives and ties
+    are theirs."""
+    g = torch.Generator().manual_seed(T * V)
+    x = torch.randn(T, K + 3, generator=g).to(DT[dtype]).cuda()[:, :K]
+    w, q, s = head_of(ctx, V, V, K)
+    tok = given(T, T, V, G)
+    if T > 2 and G:
+        tok[1] = -1
+    logits = product(*quantize64(x), q, s, torch.float32)
+    got = head_score(ctx, w, x, tok, k)
+    ctx.synchronize()
+    check_logprobs(got, logprobs64(logits, tok, k), (T, V, K))
+
+
+@pytest.mark.parametrize("T", [1, 6, 150])
+def test_head_ties_and_rows_that_are_not_numbers(ctx, T):
+    """Equal rows of the head tie; a zero row of x ties everywhere; a NaN in x
+    makes its row NaN and no other."""
+    V, K = 1300, 96
+    w, q, s = head_of(ctx, 5, V, K)
+    q[1::7], s[1::7] = q[0].clone(), s[0].clone()
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(T, K, generator=g).cuda()
+    if T > 3:
+        x[2] = 0.0
+        x[3, 5] = math.nan
+    tok = given(7, T, V, 1)
+    logits = product(*quantize64(x), q, s, torch.float32)
+    got = head_score(ctx, w, x, tok, 32)
+    ctx.synchronize()
+    check_logprobs(got, logprobs64(logits, tok, 32), T)
+
+
+@pytest.mark.parametrize("T", [1, 9, 140])
+def test_head_tokens_outside_the_vocabulary(ctx, T):
+    w, q, s = head_of(ctx, 8, 400, 64)
+    x = torch.randn(T, 64, generator=torch.Generator().manual_seed(9)).cuda()
+    tok = torch.full((T, 2), 3, dtype=torch.int32, device="cuda")
+    tok[0, 1], tok[T - 1, 0] = 400, -5
+    got = head_score(ctx, w, x, tok, 4)
+    with pytest.raises(har_cuda.HarCudaError) as e:
+        ctx.synchronize()
+    assert e.value.status == har_cuda.ERR_DEVICE
+    check_logprobs(got, logprobs64(product(*quantize64(x), q, s, torch.float32), tok, 4), T)
+
+
+@pytest.mark.parametrize("T", [1, 5, 200])
+def test_head_captured_and_replayed(ctx, T):
+    V, K = 1111, 160
+    w, q, s = head_of(ctx, 12, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(13)).cuda()
+    tok = given(14, T, V, 1)
+    need = w.head_workspace(T, 1, 7)
+    work = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+    o = outputs(T, 1, 7)
+    args = (w, x, tok, o["logprobs"], o["entropy"], o["ids"], o["top"])
+    ctx.i8_head_logprobs(*args, workspace=work)
+    torch.cuda.synchronize()
+    g, side, refused = torch.cuda.CUDAGraph(), torch.cuda.Stream(), False
+    try:
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            ctx.bind_torch_stream()
+            try:
+                ctx.i8_head_logprobs(*args)
+            except har_cuda.HarCudaError as e:
+                refused = e.status == har_cuda.ERR_ARG
+            ctx.i8_head_logprobs(*args, workspace=work)
+            g.capture_end()
+    finally:
+        ctx.bind_torch_stream()
+    assert refused == bool(need)
+    x.mul_(-1.5)
+    g.replay()
+    torch.cuda.synchronize()
+    check_logprobs(o, logprobs64(product(*quantize64(x), q, s, torch.float32), tok, 7), T)
+
+
+def test_head_refusals(ctx):
+    w, _, _ = head_of(ctx, 15, 64, 32)
+    x, tok = torch.randn(4, 32, device="cuda"), given(1, 4, 64, 1)
+    o = outputs(4, 1, 2)
+    args = (tok, o["logprobs"], o["entropy"], o["ids"], o["top"])
+
+    def refused(status, *a, **k):
+        with pytest.raises(har_cuda.HarCudaError) as e:
+            ctx.i8_head_logprobs(*a, **k)
+        assert e.value.status == status, e.value
+
+    refused(har_cuda.ERR_GEOMETRY, w, x[:, :31], *args)
+    refused(har_cuda.ERR_ARG, w, x.long(), *args)
+    refused(har_cuda.ERR_GEOMETRY, w, x, tok[:3], *args[1:])
+    refused(har_cuda.ERR_ARG, w, x, None, *args[1:])
+    refused(har_cuda.ERR_ARG, w, x, *args, workspace=torch.empty(1, dtype=torch.uint8, device="cuda"))
+    assert w.head_workspace(-1, 1, 1) == -1 and w.head_workspace(4, 1, 33) == -1
