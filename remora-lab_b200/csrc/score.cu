@@ -56,8 +56,8 @@ static int32_t check_i8_rows(har_cuda_ctx *ctx, const int8_t *q, int64_t rows, i
 }
 
 static int32_t check_nk(har_cuda_ctx *ctx, int64_t N, int64_t K, const char *who) {
-  if (N < 1 || N > INT32_MAX || K < 1 || K > I8_MAX_K)
-    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, std::string(who) + ": need 1 <= N < 2^31 and 1 <= K <= " +
+  if (N < 1 || N > I8_MAX_ROWS || K < 1 || K > I8_MAX_K)
+    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, std::string(who) + ": need 1 <= N <= 2^30 and 1 <= K <= " +
                                                      std::to_string(I8_MAX_K));
   return HAR_CUDA_OK;
 }
@@ -112,8 +112,8 @@ int32_t har_cuda_i8_quantize(har_cuda_ctx *ctx, const void *x_dev, int32_t dtype
                              float *scale_dev) {
   if (!ctx) return HAR_CUDA_ERR_ARG;
   HAR_TRY(check_dtype(ctx, dtype, "i8_quantize"));
-  if (M < 0 || M > INT32_MAX || K < 1 || K > INT32_MAX)
-    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_quantize: need 0 <= M < 2^31 and 1 <= K < 2^31");
+  if (M < 0 || M > I8_MAX_ROWS || K < 1 || K > I8_MAX_ROWS)
+    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_quantize: need 0 <= M <= 2^30 and 1 <= K <= 2^30");
   if (M == 0) return HAR_CUDA_OK;
   HAR_TRY(check_rows(ctx, x_dev, dtype_bytes(dtype), M, K, ldx, false, "i8_quantize: x"));
   HAR_TRY(check_rows(ctx, q_dev, 1, M, K, ldq, true, "i8_quantize: q"));
@@ -121,6 +121,16 @@ int32_t har_cuda_i8_quantize(har_cuda_ctx *ctx, const void *x_dev, int32_t dtype
   OnDevice on(ctx);
   HAR_TRY(on.status(ctx));
   return launch_i8_quantize(ctx, x_dev, dtype, M, K, ldx, q_dev, ldq, scale_dev);
+}
+
+static int32_t finish_i8_weights(har_cuda_ctx *ctx, har_cuda_i8_weights *w, har_cuda_i8_weights **out) {
+  const int32_t st = encode_tmap_2d(ctx, &w->map, w->q, 1, (uint64_t)w->N, (uint64_t)w->K, (uint64_t)w->ldq, 128, 128, true);
+  if (st != HAR_CUDA_OK) {
+    har_cuda_i8_weights_free(w);
+    return st;
+  }
+  *out = w;
+  return HAR_CUDA_OK;
 }
 
 int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32_t dtype,
@@ -153,8 +163,7 @@ int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32
   w->q = (const int8_t *)d;
   w->scale = (const float *)((uint8_t *)d + qb);
   w->N = N, w->K = K, w->ldq = ldq, w->device = ctx->device, w->owned = true;
-  *out = w;
-  return HAR_CUDA_OK;
+  return finish_i8_weights(ctx, w, out);
 }
 
 int32_t har_cuda_i8_weights_wrap(har_cuda_ctx *ctx, const int8_t *q_dev, int64_t ldq,
@@ -170,8 +179,7 @@ int32_t har_cuda_i8_weights_wrap(har_cuda_ctx *ctx, const int8_t *q_dev, int64_t
   w->q = q_dev;
   w->scale = scale_dev;
   w->N = N, w->K = K, w->ldq = N == 1 ? (int64_t)round16((size_t)K) : ldq, w->device = ctx->device;
-  *out = w;
-  return HAR_CUDA_OK;
+  return finish_i8_weights(ctx, w, out);
 }
 
 int32_t har_cuda_i8_weights_free(har_cuda_i8_weights *w) {
@@ -193,7 +201,7 @@ int32_t har_cuda_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
   if (!ctx) return HAR_CUDA_ERR_ARG;
   HAR_TRY(check_i8_weights(ctx, w, "i8_matmul"));
   HAR_TRY(check_dtype(ctx, y_dtype, "i8_matmul"));
-  if (M < 0 || M > INT32_MAX) return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_matmul: need 0 <= M < 2^31");
+  if (M < 0 || M > I8_MAX_ROWS) return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_matmul: need 0 <= M <= 2^30");
   if (M == 0) return HAR_CUDA_OK;
   HAR_TRY(check_i8_rows(ctx, q_dev, M, w->K, ldq, "i8_matmul: q"));
   HAR_TRY(check_rows(ctx, scale_dev, 4, 1, M, M, false, "i8_matmul: scale"));
@@ -210,7 +218,7 @@ static size_t quantized_bytes(const har_cuda_i8_weights *w, int64_t M) {
 }
 
 int64_t har_cuda_i8_linear_workspace(const har_cuda_i8_weights *w, int64_t M) {
-  if (!w || M < 0 || M > INT32_MAX) return -1;
+  if (!w || M < 0 || M > I8_MAX_ROWS) return -1;
   return M == 0 ? 0 : (int64_t)quantized_bytes(w, M);
 }
 
@@ -221,7 +229,7 @@ int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
   HAR_TRY(check_i8_weights(ctx, w, "i8_linear"));
   HAR_TRY(check_dtype(ctx, x_dtype, "i8_linear"));
   HAR_TRY(check_dtype(ctx, y_dtype, "i8_linear"));
-  if (M < 0 || M > INT32_MAX) return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_linear: need 0 <= M < 2^31");
+  if (M < 0 || M > I8_MAX_ROWS) return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, "i8_linear: need 0 <= M <= 2^30");
   if (M == 0) return HAR_CUDA_OK;
   HAR_TRY(check_rows(ctx, x_dev, dtype_bytes(x_dtype), M, w->K, ldx, false, "i8_linear: x"));
   HAR_TRY(check_rows(ctx, y_dev, dtype_bytes(y_dtype), M, w->N, ldy, true, "i8_linear: y"));
@@ -239,8 +247,8 @@ int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
 
 static int32_t check_logprobs(har_cuda_ctx *ctx, int64_t T, int64_t V, const LogprobOut &o, const char *name) {
   const std::string who(name);
-  if (T < 0 || T > INT32_MAX || V < 1 || V > INT32_MAX)
-    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, who + ": need 0 <= T < 2^31 and 1 <= V < 2^31");
+  if (T < 0 || T > I8_MAX_ROWS || V < 1 || V > I8_MAX_ROWS)
+    return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, who + ": need 0 <= T <= 2^30 and 1 <= V <= 2^30");
   if (o.G < 0 || o.k < 0 || o.k > I8_MAX_TOP)
     return set_error(ctx, HAR_CUDA_ERR_GEOMETRY, who + ": need G >= 0 and 0 <= k <= " + std::to_string(I8_MAX_TOP));
   if (T == 0) return HAR_CUDA_OK;
@@ -270,7 +278,7 @@ int32_t har_cuda_token_logprobs(har_cuda_ctx *ctx, const void *logits_dev, int32
 static int64_t head_rows(int64_t T) { return T < 128 ? T : 128; }
 
 int64_t har_cuda_i8_head_workspace(const har_cuda_i8_weights *w, int64_t T, int32_t G, int32_t k) {
-  if (!w || T < 0 || T > INT32_MAX || G < 0 || k < 0 || k > I8_MAX_TOP) return -1;
+  if (!w || T < 0 || T > I8_MAX_ROWS || G < 0 || k < 0 || k > I8_MAX_TOP) return -1;
   if (T == 0) return 0;
   return (int64_t)(quantized_bytes(w, T) + (size_t)head_rows(T) * (size_t)w->N * sizeof(float));
 }

@@ -14,6 +14,8 @@ struct har_cuda_i8_weights {
   int64_t N = 0, K = 0, ldq = 0;
   int device = 0;
   bool owned = false;  // q and scale share one allocation, at q
+  // TMA map of q for the tensor-core kernels: boxes of 128 rows x 128 bytes
+  TmaDesc map;
 };
 
 namespace har {
@@ -21,6 +23,7 @@ namespace har {
 // Longest row whose integer sum fits in 32 bits with every product at its
 // largest, 128 * 128: 131,071, rounded down to whole 16-byte pieces.
 constexpr int64_t I8_MAX_K = 131056;
+constexpr int64_t I8_MAX_ROWS = (int64_t)1 << 30;  // row numbers, tiles included, fit in 32 bits
 constexpr int I8_MAX_TOP = HAR_CUDA_LOGPROBS_MAX_TOP;
 
 inline size_t dtype_bytes(int32_t dtype) { return dtype == HAR_CUDA_DTYPE_F32 ? 4 : 2; }
