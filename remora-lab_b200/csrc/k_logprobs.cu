@@ -1,100 +1,343 @@
 // k_logprobs.cu — log probabilities of given tokens, entropy and the largest
-// alternatives of each row of logits.
-#include "score.cuh"
+// alternatives of each row of logits, in one pass over the row:
+//   s = sum exp(x - r),  t = sum exp(x - r) (x - r)  for a reference r near the
+// row's maximum, so log p = (x - r) - log s and H = log s - t / s whatever r is.
+#include <algorithm>
+#include <cooperative_groups.h>
+
+#include "topk_warp.cuh"
 
 namespace har {
 
-// Running sums of a softmax: m the largest logit, s = sum exp(x - m),
-// t = sum exp(x - m) (x - m).  A logit of -inf adds nothing.
-struct Stat {
-  float m, s, t;
-};
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.t + b.t};  // both empty, or NaN kept in the sums
-  auto part = [m](Stat c, float &s, float &t) {
-    if (c.m == -INFINITY) {
-      s = c.s, t = c.t;
-      return;
-    }
-    const float d = c.m - m, e = expf(d);
-    s = c.s * e;
-    t = e == 0.0f ? 0.0f * c.t : e * (c.t + d * c.s);
-  };
-  float s1, t1, s2, t2;
-  part(a, s1, t1);
-  part(b, s2, t2);
-  return {m, s1 + s2, t1 + t2};
+namespace cg = cooperative_groups;
+
+constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_MAX_CLUSTER = 16;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256)
-    token_logprobs_kernel(const T *__restrict__ x, int64_t V, int64_t ldl, LogprobOut out) {
-  __shared__ Stat stats[8];
-  __shared__ unsigned long long keys[8];
-  const int64_t row = blockIdx.x;
-  const T *xr = x + row * ldl;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Stat st = {-INFINITY, 0.0f, 0.0f};
-  for (int64_t i = threadIdx.x; i < V; i += 256) {
-    const float v = to_f32(xr[i]);
-    if (v != -INFINITY) st = stat_merge(st, {v, v != v ? v : 1.0f, 0.0f});
+// Sums about a reference: r starts at -inf (nothing seen but -inf and NaN).
+struct Stat {
+  float r, s, t;
+};
+// Moves the sums to reference r (>= a.r).  From -inf the sums are 0, or NaN.
+__device__ __forceinline__ void stat_move(Stat &a, float r) {
+  if (a.r == r) return;
+  const float d = a.r - r, f = ex2(d * LOG2E);
+  const float shift = a.r == -INFINITY ? 0.0f : f == 0.0f ? 0.0f : d;
+  a.t = f * fmaf(shift, a.s, a.t);
+  a.s = f * a.s;
+  a.r = r;
+}
+__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
+  const float r = fmaxf(a.r, b.r);
+  stat_move(a, r);
+  stat_move(b, r);
+  return {r, a.s + b.s, a.t + b.t};
+}
+__device__ __forceinline__ Stat warp_stat(Stat a) {
+  float r = a.r;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
+  stat_move(a, r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
   }
-  for (int o = 16; o; o >>= 1) {
-    Stat b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o), __shfl_xor_sync(~0u, st.t, o)};
-    st = stat_merge(st, b);
+  return a;
+}
+
+// One 16-byte piece of a row.
+template <typename T>
+struct Piece {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 raw;
+  // elements e0 .. e0 + N - 1 of the row at x, whole pieces with one load; an
+  // element outside [0, V) reads as -inf, which adds nothing to the sums
+  __device__ __forceinline__ void load(const T *x, int64_t e0, int64_t V) {
+    if (e0 >= 0 && e0 + N <= V) {
+      raw = ldg_nc_v4(x + e0);
+    } else {
+      T v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < V ? x[e0 + i] : from_f32<T>(-INFINITY);
+      raw = *reinterpret_cast<const uint4 *>(v);
+    }
+  }
+  __device__ __forceinline__ void none() {
+    T v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = from_f32<T>(-INFINITY);
+    raw = *reinterpret_cast<const uint4 *>(v);
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f32(reinterpret_cast<const T *>(&raw)[i]); }
+  // largest element, NaN left out
+  __device__ __forceinline__ float top() const;
+};
+template <>
+__device__ __forceinline__ float Piece<float>::top() const {
+  return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
+}
+template <>
+__device__ __forceinline__ float Piece<__half>::top() const {
+  const __half2 *v = reinterpret_cast<const __half2 *>(&raw);
+  const __half2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+  return __half2float(__hmax(__low2half(m), __high2half(m)));
+}
+template <>
+__device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
+  const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&raw);
+  const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+  return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
+}
+
+// Adds a piece to the sums.  The reference follows the maximum only once it is
+// left behind by more than 6 (e^6 = 403 a term at most): a move costs an
+// exponential, and close behind the maximum it would run at almost every piece.
+template <typename T>
+__device__ __forceinline__ void stat_add(Stat &a, const Piece<T> &p, float top) {
+  if (top > a.r + 6.0f) stat_move(a, top);
+  const float r = a.r == -INFINITY ? 0.0f : a.r;
+  const float2 nr = make_float2(-r, -r), l2e = make_float2(LOG2E, LOG2E);
+  float2 s = make_float2(a.s, 0.0f), t = make_float2(a.t, 0.0f);
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N; i += 2) {
+    float2 d = __fadd2_rn(make_float2(p.at(i), p.at(i + 1)), nr);
+    d.x = max_nan(d.x, -1e4f);  // -inf (0 times it would be NaN) and all that underflows
+    d.y = max_nan(d.y, -1e4f);
+    const float2 g = __fmul2_rn(d, l2e);
+    const float2 e = make_float2(ex2(g.x), ex2(g.y));
+    s = __fadd2_rn(s, e);
+    t = __ffma2_rn(e, d, t);
+  }
+  a.s = s.x + s.y;
+  a.t = t.x + t.y;
+}
+
+// A warp's candidates: keys above `limit` wait in a shared buffer until 32 are
+// there, then one sort and one merge take them into the list.  Elements come
+// in ascending order, step by step (32 lanes x one piece), so once the list
+// holds k entries a value equal to the last of them loses to it: `bar` is that
+// value, or NaN while there is no such entry.
+struct Alternatives {
+  key_t list, limit;
+  float bar;
+  key_t *buf;  // 32 + 32 * 8 keys
+  int *count;
+  int k, lane;
+
+  __device__ __forceinline__ void init(key_t *buf_, int *count_, int k_, int lane_) {
+    list = 0, limit = 0, bar = __int_as_float(0x7fffffff), buf = buf_, count = count_, k = k_, lane = lane_;
+    if (lane == 0) *count = 0;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void push(float v, int64_t id) {
+    const key_t key = order_key(v, (uint32_t)id);
+    if (key > limit) buf[atomicAdd(count, 1)] = key;
+  }
+  // takes the waiting candidates in; the whole warp, converged
+  __device__ __forceinline__ void drain(int least) {
+    __syncwarp();
+    const int n = *reinterpret_cast<volatile int *>(count);
+    if (n < least || n == 0) return;
+    for (int i = 0; i < n; i += 32)
+      list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? buf[i + lane] : 0, lane), lane);
+    __syncwarp();
+    if (lane == 0) *count = 0;
+    const key_t last = __shfl_sync(0xffffffffu, list, k - 1);
+    if (last) {
+      limit = key_max(limit, last);
+      bar = order_value((uint32_t)(last >> 32));
+    }
+    __syncwarp();
+  }
+};
+
+// A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
+// part of its pieces.
+template <typename T>
+__global__ void __launch_bounds__(LP_T, 4)
+    token_logprobs_kernel(const T *__restrict__ logits, int64_t V, int64_t ldl, LogprobOut out, int C) {
+  constexpr int N = Piece<T>::N;
+  __shared__ key_t bufs[LP_WARPS][32 + 32 * N];
+  __shared__ int counts[LP_WARPS];
+  __shared__ key_t lists[LP_MAX_CLUSTER][32];   // the block's lists, then the cluster's
+  __shared__ key_t part_list[LP_WARPS][32];
+  __shared__ Stat stats[LP_WARPS], part_stats[LP_MAX_CLUSTER];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x / C;
+  const int rank = (int)(blockIdx.x - row * C);
+  const T *x = logits + row * ldl;
+  const bool want_top = out.k > 0 && (out.top_ids || out.top_logprobs);
+  if (C > 1) cg::this_cluster().barrier_arrive();
+
+  // the first given tokens' logits are asked for before anything else
+  int32_t tok = -1;
+  float given = 0.0f;
+  const bool has_given = rank == 0 && out.logprobs && (int)threadIdx.x < out.G;
+  if (has_given) {
+    tok = out.tokens[row * out.G + threadIdx.x];
+    if (tok >= 0 && tok < V) given = to_f32(x[tok]);
+  }
+
+  // pieces are 16-byte aligned: the first may start before the row
+  const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
+  const int64_t pieces = (V + off + N - 1) / N, share = (pieces + C - 1) / C;
+  const int64_t j0 = rank * share, j1 = min(pieces, j0 + share);
+  Stat st = {-INFINITY, 0.0f, 0.0f};
+  Alternatives alt;
+  alt.init(bufs[warp], counts + warp, out.k, lane);
+  for (int64_t jw = j0 + 32 * warp; jw < j1; jw += LP_T * LP_U) {  // the same trips for a warp's lanes
+    Piece<T> p[LP_U];
+    float top[LP_U];
+#pragma unroll
+    for (int u = 0; u < LP_U; ++u) {
+      const int64_t j = jw + lane + u * LP_T;
+      if (j < j1) p[u].load(x, j * N - off, V);
+      else p[u].none();
+    }
+#pragma unroll
+    for (int u = 0; u < LP_U; ++u) top[u] = p[u].top();
+    if (want_top && jw == j0 + 32 * warp) {
+      // the k-th largest of the lanes' largest values: k elements are at least
+      // as large, so nothing below it is worth a place (-inf may be filling)
+      float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const key_t kth = __shfl_sync(0xffffffffu, warp_sort_desc((key_t)order_bits(m) << 32, lane), out.k - 1);
+      alt.limit = kth > (key_t)order_bits(-INFINITY) << 32 ? kth : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < LP_U; ++u) {
+      if (want_top) {
+        const bool pass = !(top[u] <= alt.bar);
+        if (__any_sync(0xffffffffu, pass)) {
+          const int64_t j = jw + lane + u * LP_T, e0 = j * N - off;
+          if (pass && j < j1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (e0 + i >= 0 && e0 + i < V) alt.push(p[u].at(i), e0 + i);
+          }
+          alt.drain(32);
+        }
+      }
+      stat_add(st, p[u], top[u]);
+    }
+    if (want_top && jw == j0 + 32 * warp) alt.drain(1);
+  }
+  st = warp_stat(st);
+  if (want_top) {
+    alt.drain(1);
+    part_list[warp][lane] = alt.list;
   }
   if (lane == 0) stats[warp] = st;
   __syncthreads();
-  st = stats[0];
-  for (int w = 1; w < 8; ++w) st = stat_merge(st, stats[w]);
-  const bool empty = st.m == -INFINITY && !(st.s != st.s);
+  key_t best = want_top ? block_merge_lists(part_list, LP_WARPS, warp, lane) : 0;
+  if (warp == 0) st = warp_stat(lane < LP_WARPS ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+  if (C > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.barrier_wait();  // every block of the cluster has started: its shared memory is there
+    if (warp == 0) {
+      *cl.map_shared_rank(&lists[rank][lane], 0) = best;
+      if (lane == 0) *cl.map_shared_rank(&part_stats[rank], 0) = st;
+    }
+    cl.sync();
+    if (rank != 0) return;
+    if (want_top) best = block_merge_lists(lists, C, warp, lane);
+    st = warp_stat(lane < C ? part_stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+  } else {
+    if (warp == 0 && lane == 0) part_stats[0] = st;
+    __syncthreads();
+    st = part_stats[0];
+  }
+
+  // an empty row has no reference; a NaN or +inf makes s NaN
+  const bool empty = st.r == -INFINITY && st.s == 0.0f;
   const float logz = empty ? 0.0f : logf(st.s);
-  auto logp = [&](float v) { return empty ? -INFINITY : (v - st.m) - logz; };
+  auto logp = [&](float v) { return empty ? -INFINITY : (v - st.r) - logz; };
   if (threadIdx.x == 0 && out.entropy) out.entropy[row] = empty ? 0.0f : logz - st.t / st.s;
   if (out.logprobs)
-    for (int g = threadIdx.x; g < out.G; g += 256) {
-      const int32_t tok = out.tokens[row * out.G + g];
+    for (int g = threadIdx.x; g < out.G; g += LP_T) {
+      if (g >= LP_T) {
+        tok = out.tokens[row * out.G + g];
+        if (tok >= 0 && tok < V) given = to_f32(x[tok]);
+      }
       float r = 0.0f;
       if (tok >= 0 && tok < V) {
-        r = logp(to_f32(xr[tok]));
+        r = logp(given);
       } else if (tok != -1) {
         r = __int_as_float(0x7fffffff);
         atomicOr(out.status, DEV_ERR_BOUNDS);
       }
       out.logprobs[row * out.G + g] = r;
     }
-  if (!out.top_ids && !out.top_logprobs) return;
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < out.k; ++j) {
-    unsigned long long best = 0;
-    for (int64_t i = threadIdx.x; i < V; i += 256) {
-      const unsigned long long key = order_key(to_f32(xr[i]), (uint32_t)i);
-      if (key < last && key > best) best = key;
-    }
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-    __syncthreads();
-    if (lane == 0) keys[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) best = max(best, keys[w]);
-    last = best;
-    if (threadIdx.x == 0) {
-      if (out.top_ids) out.top_ids[row * out.k + j] = best ? (int32_t)(0xffffffffu - (uint32_t)best) : -1;
-      if (out.top_logprobs)
-        out.top_logprobs[row * out.k + j] =
-            st.s != st.s ? st.s : best ? logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
-    }
+  if (want_top && warp == 0 && lane < out.k) {
+    const int64_t o = row * out.k + lane;
+    if (out.top_ids) out.top_ids[o] = best ? (int32_t)(0xffffffffu - (uint32_t)best) : -1;
+    if (out.top_logprobs)
+      out.top_logprobs[o] = st.s != st.s ? st.s : best ? logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
   }
+}
+
+// Blocks a row: 1 to 16, a power of two.  592 blocks (4 an SM) run at a time;
+// a block costs its share of the row and about 4,096 elements' time to start
+// and to join.
+static int pick_cluster(int64_t T, int64_t V, int sms) {
+  int best = 1;
+  double least = 0;
+  for (int c = 1; c <= LP_MAX_CLUSTER; c *= 2) {
+    const int64_t waves = (T * c + 4 * sms - 1) / (4 * sms);
+    const double cost = (double)waves * ((double)V / c + 4096.0);
+    if (c == 1 || cost < least) best = c, least = cost;
+  }
+  return best;
 }
 
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
                               int64_t V, int64_t ldl, const LogprobOut &out) {
-  prof_begin(ctx);
-  with_dtype(dtype, [&](auto t) {
-    using E = decltype(t);
-    token_logprobs_kernel<E><<<(unsigned)T, 256, 0, ctx->stream>>>((const E *)logits, V, ldl, out);
-  });
-  return check_launch(ctx, "token_logprobs_kernel");
+  const int C = pick_cluster(T, V, ctx->num_sms);
+  cudaError_t e = cudaSuccess;
+  // a grid holds 2^31 - 1 blocks
+  const int64_t most = ((int64_t)1 << 30) / C;
+  for (int64_t t0 = 0; t0 < T; t0 += most) {
+    const int64_t rows = std::min(most, T - t0);
+    LogprobOut o = out;
+    if (o.tokens) o.tokens += t0 * o.G;
+    if (o.logprobs) o.logprobs += t0 * o.G;
+    if (o.entropy) o.entropy += t0;
+    if (o.top_ids) o.top_ids += t0 * o.k;
+    if (o.top_logprobs) o.top_logprobs += t0 * o.k;
+    prof_begin(ctx);
+    with_dtype(dtype, [&](auto t) {
+      using E = decltype(t);
+      if (C > 8) e = cudaFuncSetAttribute(token_logprobs_kernel<E>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(rows * C));
+      cfg.blockDim = dim3(LP_T);
+      cfg.stream = ctx->stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)C;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = C > 1 ? 1 : 0;
+      e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<E>, (const E *)logits + t0 * ldl, V, ldl, o, C);
+    });
+    const int32_t st = check_launch(ctx, "token_logprobs_kernel");
+    if (e != cudaSuccess)
+      return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("token_logprobs_kernel: ") + cudaGetErrorString(e));
+    if (st != HAR_CUDA_OK) return st;
+  }
+  return HAR_CUDA_OK;
 }
 
 }  // namespace har

@@ -278,3 +278,17 @@ def test_head_refusals(ctx):
     refused(har_cuda.ERR_ARG, w, x, None, *args[1:])
     refused(har_cuda.ERR_ARG, w, x, *args, workspace=torch.empty(1, dtype=torch.uint8, device="cuda"))
     assert w.head_workspace(-1, 1, 1) == -1 and w.head_workspace(4, 1, 33) == -1
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rows_of_a_few_values_that_are_not_numbers(ctx, dtype):
+    """Rows shorter than a warp's first trip with NaN among them: filling must
+    not take an element's place."""
+    for V in (1, 3, 9, 40):
+        x = logits_of(V, 4, V, dtype, pad=1)
+        x[0] = math.nan
+        x[1, 0] = math.nan
+        x[2] = -math.inf
+        x[2, V // 2] = math.nan
+        tok = given(1, 4, V, 1)
+        check_logprobs(score(ctx, x, tok, 32), logprobs64(x, tok, 32), (dtype, V))
