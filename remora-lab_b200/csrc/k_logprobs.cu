@@ -11,7 +11,7 @@ namespace har {
 
 namespace cg = cooperative_groups;
 
-constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_MAX_CLUSTER = 16;
+constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_SEG = 32, LP_MAX_CLUSTER = 16;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float v) {
@@ -101,80 +101,50 @@ __device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
   return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
 }
 
-// Adds a piece to the sums.  The reference follows the maximum only once it is
-// left behind by more than 6 (e^6 = 403 a term at most): a move costs an
-// exponential, and close behind the maximum it would run at almost every piece.
+// Adds a trip's pieces, whose largest element is `top`, to the sums.  The
+// reference follows the maximum only once it is left behind by more than 6
+// (e^6 = 403 a term at most): a move costs an exponential, and close behind
+// the maximum it would run at almost every trip.
 template <typename T>
-__device__ __forceinline__ void stat_add(Stat &a, const Piece<T> &p, float top) {
+__device__ __forceinline__ void stat_add(Stat &a, const Piece<T> (&p)[LP_U], float top) {
   if (top > a.r + 6.0f) stat_move(a, top);
   const float r = a.r == -INFINITY ? 0.0f : a.r;
   const float2 nr = make_float2(-r, -r), l2e = make_float2(LOG2E, LOG2E);
   float2 s = make_float2(a.s, 0.0f), t = make_float2(a.t, 0.0f);
 #pragma unroll
-  for (int i = 0; i < Piece<T>::N; i += 2) {
-    float2 d = __fadd2_rn(make_float2(p.at(i), p.at(i + 1)), nr);
-    d.x = max_nan(d.x, -1e4f);  // -inf (0 times it would be NaN) and all that underflows
-    d.y = max_nan(d.y, -1e4f);
-    const float2 g = __fmul2_rn(d, l2e);
-    const float2 e = make_float2(ex2(g.x), ex2(g.y));
-    s = __fadd2_rn(s, e);
-    t = __ffma2_rn(e, d, t);
-  }
+  for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+    for (int i = 0; i < Piece<T>::N; i += 2) {
+      float2 d = __fadd2_rn(make_float2(p[u].at(i), p[u].at(i + 1)), nr);
+      d.x = max_nan(d.x, -1e4f);  // -inf (0 times it would be NaN) and all that underflows
+      d.y = max_nan(d.y, -1e4f);
+      const float2 g = __fmul2_rn(d, l2e);
+      const float2 e = make_float2(ex2(g.x), ex2(g.y));
+      s = __fadd2_rn(s, e);
+      t = __ffma2_rn(e, d, t);
+    }
   a.s = s.x + s.y;
   a.t = t.x + t.y;
 }
 
-// A warp's candidates: keys above `limit` wait in a shared buffer until 32 are
-// there, then one sort and one merge take them into the list.  Elements come
-// in ascending order, step by step (32 lanes x one piece), so once the list
-// holds k entries a value equal to the last of them loses to it: `bar` is that
-// value, or NaN while there is no such entry.
-struct Alternatives {
-  key_t list, limit;
-  float bar;
-  key_t *buf;  // 32 + 32 * 8 keys
-  int *count;
-  int k, lane;
-
-  __device__ __forceinline__ void init(key_t *buf_, int *count_, int k_, int lane_) {
-    list = 0, limit = 0, bar = __int_as_float(0x7fffffff), buf = buf_, count = count_, k = k_, lane = lane_;
-    if (lane == 0) *count = 0;
-    __syncwarp();
-  }
-  __device__ __forceinline__ void push(float v, int64_t id) {
-    const key_t key = order_key(v, (uint32_t)id);
-    if (key > limit) buf[atomicAdd(count, 1)] = key;
-  }
-  // takes the waiting candidates in; the whole warp, converged
-  __device__ __forceinline__ void drain(int least) {
-    __syncwarp();
-    const int n = *reinterpret_cast<volatile int *>(count);
-    if (n < least || n == 0) return;
-    for (int i = 0; i < n; i += 32)
-      list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? buf[i + lane] : 0, lane), lane);
-    __syncwarp();
-    if (lane == 0) *count = 0;
-    const key_t last = __shfl_sync(0xffffffffu, list, k - 1);
-    if (last) {
-      limit = key_max(limit, last);
-      bar = order_value((uint32_t)(last >> 32));
-    }
-    __syncwarp();
-  }
-};
-
 // A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
-// part of its pieces.
+// part of its pieces, walked in trips of LP_T x LP_U pieces.  The alternatives
+// cost the walk one store: a thread notes the largest element of each trip (a
+// group of LP_U pieces).  After up to LP_SEG trips the k-th largest of the
+// threads' largest elements bounds the k-th largest of all from below, so only
+// groups that reach it (about k of thousands) can hold an alternative; a warp
+// reads its own again, from L2, one element a lane, into its sorted list.
 template <typename T>
 __global__ void __launch_bounds__(LP_T, 4)
     token_logprobs_kernel(const T *__restrict__ logits, int64_t V, int64_t ldl, LogprobOut out, int C) {
   constexpr int N = Piece<T>::N;
-  __shared__ key_t bufs[LP_WARPS][32 + 32 * N];
-  __shared__ int counts[LP_WARPS];
-  __shared__ key_t lists[LP_MAX_CLUSTER][32];   // the block's lists, then the cluster's
+  __shared__ float group_top[LP_SEG][LP_T];
+  __shared__ uint32_t tops[LP_WARPS][32];
+  __shared__ uint32_t bound_s;
+  __shared__ key_t lists[LP_MAX_CLUSTER][32];  // the block's lists, then the cluster's
   __shared__ key_t part_list[LP_WARPS][32];
   __shared__ Stat stats[LP_WARPS], part_stats[LP_MAX_CLUSTER];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / C;
   const int rank = (int)(blockIdx.x - row * C);
   const T *x = logits + row * ldl;
@@ -184,9 +154,8 @@ __global__ void __launch_bounds__(LP_T, 4)
   // the first given tokens' logits are asked for before anything else
   int32_t tok = -1;
   float given = 0.0f;
-  const bool has_given = rank == 0 && out.logprobs && (int)threadIdx.x < out.G;
-  if (has_given) {
-    tok = out.tokens[row * out.G + threadIdx.x];
+  if (rank == 0 && out.logprobs && tid < out.G) {
+    tok = out.tokens[row * out.G + tid];
     if (tok >= 0 && tok < V) given = to_f32(x[tok]);
   }
 
@@ -194,50 +163,73 @@ __global__ void __launch_bounds__(LP_T, 4)
   const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
   const int64_t pieces = (V + off + N - 1) / N, share = (pieces + C - 1) / C;
   const int64_t j0 = rank * share, j1 = min(pieces, j0 + share);
-  Stat st = {-INFINITY, 0.0f, 0.0f};
-  Alternatives alt;
-  alt.init(bufs[warp], counts + warp, out.k, lane);
-  for (int64_t jw = j0 + 32 * warp; jw < j1; jw += LP_T * LP_U) {  // the same trips for a warp's lanes
-    Piece<T> p[LP_U];
-    float top[LP_U];
+  const int64_t whole0 = off ? 1 : 0, whole1 = min(j1, (V + off) / N);  // pieces inside the row
+  auto load_trip = [&](Piece<T>(&p)[LP_U], int64_t jt) {
+    if (jt >= whole0 && jt + LP_T * LP_U <= whole1) {
+      const T *at = x + (jt + tid) * N - off;
 #pragma unroll
-    for (int u = 0; u < LP_U; ++u) {
-      const int64_t j = jw + lane + u * LP_T;
-      if (j < j1) p[u].load(x, j * N - off, V);
-      else p[u].none();
-    }
+      for (int u = 0; u < LP_U; ++u) p[u].raw = ldg_nc_v4(at + u * LP_T * N);
+    } else {
 #pragma unroll
-    for (int u = 0; u < LP_U; ++u) top[u] = p[u].top();
-    if (want_top && jw == j0 + 32 * warp) {
-      // the k-th largest of the lanes' largest values: k elements are at least
-      // as large, so nothing below it is worth a place (-inf may be filling)
-      float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      const key_t kth = __shfl_sync(0xffffffffu, warp_sort_desc((key_t)order_bits(m) << 32, lane), out.k - 1);
-      alt.limit = kth > (key_t)order_bits(-INFINITY) << 32 ? kth : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < LP_U; ++u) {
-      if (want_top) {
-        const bool pass = !(top[u] <= alt.bar);
-        if (__any_sync(0xffffffffu, pass)) {
-          const int64_t j = jw + lane + u * LP_T, e0 = j * N - off;
-          if (pass && j < j1) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-              if (e0 + i >= 0 && e0 + i < V) alt.push(p[u].at(i), e0 + i);
-          }
-          alt.drain(32);
-        }
+      for (int u = 0; u < LP_U; ++u) {
+        const int64_t j = jt + tid + u * LP_T;
+        if (j < j1) p[u].load(x, j * N - off, V);
+        else p[u].none();
       }
-      stat_add(st, p[u], top[u]);
     }
-    if (want_top && jw == j0 + 32 * warp) alt.drain(1);
+  };
+  Stat st = {-INFINITY, 0.0f, 0.0f};
+  key_t list = 0;
+  float bar = -INFINITY;  // the k-th entry's value, once there are k
+  Piece<T> next[LP_U];
+  if (j0 < j1) load_trip(next, j0);
+  for (int64_t seg = j0; seg < j1; seg += (int64_t)LP_SEG * LP_T * LP_U) {
+    float most = -INFINITY;
+    const int trips = (int)min((int64_t)LP_SEG, (j1 - seg + LP_T * LP_U - 1) / (LP_T * LP_U));
+    for (int s = 0; s < trips; ++s) {
+      Piece<T> p[LP_U];
+#pragma unroll
+      for (int u = 0; u < LP_U; ++u) p[u] = next[u];
+      const int64_t jn = seg + (int64_t)(s + 1) * (LP_T * LP_U);
+      if (jn < j1) load_trip(next, jn);
+      float top = p[0].top();
+#pragma unroll
+      for (int u = 1; u < LP_U; ++u) top = fmaxf(top, p[u].top());
+      group_top[s][tid] = top;
+      most = fmaxf(most, top);
+      stat_add(st, p, top);
+    }
+    if (!want_top) continue;
+    // the bound: -inf itself never enters (an empty place is filled at the end)
+    tops[warp][lane] = warp_sort_desc(order_bits(most), lane);
+    __syncthreads();
+    const uint32_t merged = block_merge_lists(tops, LP_WARPS, warp, lane);
+    if (warp == 0 && lane == out.k - 1) bound_s = max(merged, order_bits(-INFINITY) + 1u);
+    __syncthreads();
+    const uint32_t bound = bound_s;
+    if (__any_sync(0xffffffffu, order_bits(most) >= bound)) {
+      for (int s = 0; s < trips; ++s) {
+        const float top = group_top[s][tid];
+        // trips come in ascending order: a value equal to the k-th entry of
+        // the trips before loses to it
+        uint32_t groups = __ballot_sync(0xffffffffu, order_bits(top) >= bound && top > bar);
+        if (!groups) continue;
+        for (; groups; groups &= groups - 1) {
+          const int64_t j = seg + (int64_t)s * (LP_T * LP_U) + 32 * warp + (__ffs(groups) - 1) + (lane / N) * LP_T;
+          const int64_t e = j * N - off + lane % N;
+          const bool in = lane < LP_U * N && j < j1 && e >= 0 && e < V;
+          const float v = in ? to_f32(x[e]) : -INFINITY;
+          const key_t key = order_key(v, (uint32_t)e);
+          const key_t last = __shfl_sync(0xffffffffu, list, out.k - 1);
+          list = warp_take(list, key, __ballot_sync(0xffffffffu, v > -INFINITY && key > last), lane);
+        }
+        const key_t last = __shfl_sync(0xffffffffu, list, out.k - 1);
+        if (last) bar = order_value((uint32_t)(last >> 32));
+      }
+    }
   }
   st = warp_stat(st);
-  if (want_top) {
-    alt.drain(1);
-    part_list[warp][lane] = alt.list;
-  }
+  if (want_top) part_list[warp][lane] = list;
   if (lane == 0) stats[warp] = st;
   __syncthreads();
   key_t best = want_top ? block_merge_lists(part_list, LP_WARPS, warp, lane) : 0;
@@ -254,7 +246,7 @@ __global__ void __launch_bounds__(LP_T, 4)
     if (want_top) best = block_merge_lists(lists, C, warp, lane);
     st = warp_stat(lane < C ? part_stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
   } else {
-    if (warp == 0 && lane == 0) part_stats[0] = st;
+    if (tid == 0) part_stats[0] = st;
     __syncthreads();
     st = part_stats[0];
   }
@@ -263,9 +255,9 @@ __global__ void __launch_bounds__(LP_T, 4)
   const bool empty = st.r == -INFINITY && st.s == 0.0f;
   const float logz = empty ? 0.0f : logf(st.s);
   auto logp = [&](float v) { return empty ? -INFINITY : (v - st.r) - logz; };
-  if (threadIdx.x == 0 && out.entropy) out.entropy[row] = empty ? 0.0f : logz - st.t / st.s;
+  if (tid == 0 && out.entropy) out.entropy[row] = empty ? 0.0f : logz - st.t / st.s;
   if (out.logprobs)
-    for (int g = threadIdx.x; g < out.G; g += LP_T) {
+    for (int g = tid; g < out.G; g += LP_T) {
       if (g >= LP_T) {
         tok = out.tokens[row * out.G + g];
         if (tok >= 0 && tok < V) given = to_f32(x[tok]);
@@ -279,11 +271,23 @@ __global__ void __launch_bounds__(LP_T, 4)
       }
       out.logprobs[row * out.G + g] = r;
     }
-  if (want_top && warp == 0 && lane < out.k) {
-    const int64_t o = row * out.k + lane;
-    if (out.top_ids) out.top_ids[o] = best ? (int32_t)(0xffffffffu - (uint32_t)best) : -1;
-    if (out.top_logprobs)
-      out.top_logprobs[o] = st.s != st.s ? st.s : best ? logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
+  if (want_top && warp == 0) {
+    int id = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
+    float lp = best ? logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
+    // places left: the first masked elements, then the first NaN
+    int have = __popc(__ballot_sync(0xffffffffu, best != 0));
+    for (int pass = 0; pass < 2 && have < out.k; ++pass)
+      for (int64_t e = lane; have < out.k && e - lane < V; e += 32) {
+        const float v = e < V ? to_f32(x[e]) : 0.0f;
+        uint32_t m = __ballot_sync(0xffffffffu, e < V && (pass == 0 ? v == -INFINITY : v != v));
+        for (; m && have < out.k; m &= m - 1, ++have)
+          if (lane == have) id = (int)(e - lane) + __ffs(m) - 1;
+      }
+    if (lane < out.k) {
+      const int64_t o = row * out.k + lane;
+      if (out.top_ids) out.top_ids[o] = id;
+      if (out.top_logprobs) out.top_logprobs[o] = st.s != st.s ? st.s : lp;
+    }
   }
 }
 

@@ -1,5 +1,5 @@
-// topk_warp.cuh — a warp's running list of the 32 largest keys, one per lane
-// in descending order (0: empty), and the buffer new candidates wait in.
+// topk_warp.cuh — the 32 largest keys of many, one a lane of a warp in
+// descending order (0: no entry).
 #pragma once
 
 #include "score.cuh"
@@ -8,36 +8,53 @@ namespace har {
 
 using key_t = unsigned long long;
 
-__device__ __forceinline__ key_t key_max(key_t a, key_t b) { return a > b ? a : b; }
+template <typename K>
+__device__ __forceinline__ K key_max(K a, K b) { return a > b ? a : b; }
 
 // Descending bitonic sort of one key a lane.
-__device__ __forceinline__ key_t warp_sort_desc(key_t v, int lane) {
+template <typename K>
+__device__ __forceinline__ K warp_sort_desc(K v, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int step = size >> 1; step > 0; step >>= 1) {
-      const key_t o = __shfl_xor_sync(0xffffffffu, v, step);
+      const K o = __shfl_xor_sync(0xffffffffu, v, step);
       const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
       v = (o > v) == keep_max ? o : v;
     }
   return v;
 }
 // The 32 largest of two descending lists, descending.
-__device__ __forceinline__ key_t warp_merge_desc(key_t a, key_t b, int lane) {
-  key_t v = key_max(a, __shfl_sync(0xffffffffu, b, 31 - lane));
+template <typename K>
+__device__ __forceinline__ K warp_merge_desc(K a, K b, int lane) {
+  K v = key_max(a, __shfl_sync(0xffffffffu, b, 31 - lane));
 #pragma unroll
   for (int step = 16; step > 0; step >>= 1) {
-    const key_t o = __shfl_xor_sync(0xffffffffu, v, step);
+    const K o = __shfl_xor_sync(0xffffffffu, v, step);
     v = (o > v) == ((lane & step) == 0) ? o : v;
   }
   return v;
 }
+// Takes the keys of the lanes in `mask` into a descending list: a few one by
+// one, many with a sort and a merge.  The whole warp.
+__device__ __forceinline__ key_t warp_take(key_t list, key_t key, uint32_t mask, int lane) {
+  if (__popc(mask) > 6)
+    return warp_merge_desc(list, warp_sort_desc((mask >> lane) & 1u ? key : (key_t)0, lane), lane);
+  for (; mask; mask &= mask - 1) {
+    const key_t k = __shfl_sync(0xffffffffu, key, __ffs(mask) - 1);
+    const int pos = __popc(__ballot_sync(0xffffffffu, list > k));
+    const key_t up = __shfl_up_sync(0xffffffffu, list, 1);
+    list = lane < pos ? list : lane == pos ? k : up;
+  }
+  return list;
+}
 
 // n (a power of two, at most twice the block's warps) descending lists at
 // lists[i][32] -> their 32 largest in warp 0.  The whole block calls it, after
-// a barrier that follows the lists' writes.
-__device__ __forceinline__ key_t block_merge_lists(key_t (*lists)[32], int n, int warp, int lane) {
-  key_t v = warp < n ? lists[warp][lane] : 0;
+// a barrier that follows the lists' writes; it ends with a barrier.
+template <typename K>
+__device__ __forceinline__ K block_merge_lists(K (*lists)[32], int n, int warp, int lane) {
+  K v = warp < n ? lists[warp][lane] : (K)0;
   for (int half = n >> 1; half > 0; half >>= 1) {
     if (warp < half) {
       v = warp_merge_desc(v, lists[warp + half][lane], lane);

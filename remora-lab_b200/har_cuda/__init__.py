@@ -240,16 +240,20 @@ def _dptr(t) -> int:
     return t.data_ptr()
 
 
-_dtype_ids = None
+class _Types:
+    """torch's element types, looked up once (torch is imported late)."""
+    ids = None
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.f32, cls.i32, cls.i8 = torch.float32, torch.int32, torch.int8
+        cls.ids = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
 
 def _dtype(t, what: str) -> int:
     """HAR_CUDA_DTYPE_* of a float tensor."""
-    global _dtype_ids
-    if _dtype_ids is None:
-        import torch
-        _dtype_ids = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-    d = _dtype_ids.get(t.dtype)
+    d = _Types.ids.get(t.dtype)
     if d is None:
         raise HarCudaError(ERR_ARG, f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
     return d
@@ -258,7 +262,7 @@ def _dtype(t, what: str) -> int:
 def _matrix(t, device: int, what: str):
     """(rows, columns, device pointer, elements between rows) of a 2-D CUDA
     tensor whose rows are contiguous (a slice of a wider one will do)."""
-    if not t.is_cuda or t.get_device() != device:
+    if t.get_device() != device:  # -1: not on a GPU
         raise HarCudaError(ERR_ARG, f"{what}: expected a tensor on cuda:{device}")
     if t.dim() != 2:
         raise HarCudaError(ERR_GEOMETRY, f"{what}: expected a matrix, got {t.dim()} dimensions")
@@ -268,13 +272,13 @@ def _matrix(t, device: int, what: str):
     return rows, cols, t.data_ptr(), ld if rows > 1 else cols
 
 
-def _vector(t, device: int, dtype_name: str, shape, what: str):
+def _vector(t, device: int, dtype, shape, what: str):
     """Device pointer of a contiguous tensor of this type and shape."""
-    if not t.is_cuda or t.get_device() != device:
+    if t.get_device() != device:
         raise HarCudaError(ERR_ARG, f"{what}: expected a tensor on cuda:{device}")
-    if str(t.dtype) != dtype_name:
-        raise HarCudaError(ERR_ARG, f"{what}: expected {dtype_name}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.dtype != dtype:
+        raise HarCudaError(ERR_ARG, f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
         raise HarCudaError(ERR_GEOMETRY, f"{what}: expected shape {shape}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise HarCudaError(ERR_ARG, f"{what}: expected a contiguous tensor")
@@ -299,6 +303,7 @@ class Context:
             raise HarCudaError(st, f"ctx_create(device={device}) failed")
         self.handle = h
         self.device = device
+        _Types.load()
         if use_torch_stream:
             self.bind_torch_stream()
 
@@ -446,9 +451,9 @@ class Context:
         Mq, Kq, qp, ldq = _matrix(q, self.device, "i8_quantize: q")
         if (Mq, Kq) != (M, K):
             raise HarCudaError(ERR_GEOMETRY, "i8_quantize: x and q differ in shape")
-        if str(q.dtype) != "torch.int8":
+        if q.dtype != _Types.i8:
             raise HarCudaError(ERR_ARG, f"i8_quantize: q must be int8, got {q.dtype}")
-        sp = _vector(scale, self.device, "torch.float32", (M,), "i8_quantize: scale")
+        sp = _vector(scale, self.device, _Types.f32, (M,), "i8_quantize: scale")
         self.check(self.lib.har_cuda_i8_quantize(self.handle, xp, _dtype(x, "i8_quantize: x"), M, K, ldx,
                                                  qp, ldq, sp))
         return q, scale
@@ -466,9 +471,9 @@ class Context:
         """An existing int8 matrix q [N][K] (rows at multiples of 16 bytes) and
         its scales f32 [N] as weights; the tensors stay the caller's."""
         N, K, qp, ldq = _matrix(q, self.device, "wrap_i8: q")
-        if str(q.dtype) != "torch.int8":
+        if q.dtype != _Types.i8:
             raise HarCudaError(ERR_ARG, f"wrap_i8: q must be int8, got {q.dtype}")
-        sp = _vector(scale, self.device, "torch.float32", (N,), "wrap_i8: scale")
+        sp = _vector(scale, self.device, _Types.f32, (N,), "wrap_i8: scale")
         h = C.c_void_p()
         self.check(self.lib.har_cuda_i8_weights_wrap(self.handle, qp, ldq, sp, N, K, C.byref(h)))
         w = I8Weights(self, h, N, K)
@@ -482,9 +487,9 @@ class Context:
         My, N, yp, ldy = _matrix(y, self.device, "i8_matmul: y")
         if K != w.K or N != w.N or My != M:
             raise HarCudaError(ERR_GEOMETRY, f"i8_matmul: q [M][{w.K}], y [M][{w.N}]")
-        if str(q.dtype) != "torch.int8":
+        if q.dtype != _Types.i8:
             raise HarCudaError(ERR_ARG, f"i8_matmul: q must be int8, got {q.dtype}")
-        sp = _vector(scale, self.device, "torch.float32", (M,), "i8_matmul: scale")
+        sp = _vector(scale, self.device, _Types.f32, (M,), "i8_matmul: scale")
         self.check(self.lib.har_cuda_i8_matmul(self.handle, w.handle, qp, ldq, sp, M, yp,
                                                _dtype(y, "i8_matmul: y"), ldy))
         return y
@@ -492,7 +497,7 @@ class Context:
     def _workspace(self, t, what: str):
         if t is None:
             return None, 0
-        if not t.is_cuda or t.get_device() != self.device or not t.is_contiguous():
+        if t.get_device() != self.device or not t.is_contiguous():
             raise HarCudaError(ERR_ARG, f"{what}: the workspace must be contiguous on cuda:{self.device}")
         return t.data_ptr(), t.numel() * t.element_size()
 
@@ -515,13 +520,13 @@ class Context:
         dev = self.device
         G = 0 if tokens is None else tokens.shape[1] if tokens.dim() == 2 else -1
         k = top_ids.shape[-1] if top_ids is not None else top_logprobs.shape[-1] if top_logprobs is not None else 0
-        tp = None if tokens is None else _vector(tokens, dev, "torch.int32", (T, G), f"{what}: tokens")
+        tp = None if tokens is None else _vector(tokens, dev, _Types.i32, (T, G), f"{what}: tokens")
         if logprobs is not None and tokens is None:
             raise HarCudaError(ERR_ARG, f"{what}: log probabilities need tokens")
-        lp = None if logprobs is None else _vector(logprobs, dev, "torch.float32", (T, G), f"{what}: logprobs")
-        ep = None if entropy is None else _vector(entropy, dev, "torch.float32", (T,), f"{what}: entropy")
-        ip = None if top_ids is None else _vector(top_ids, dev, "torch.int32", (T, k), f"{what}: top_ids")
-        bp = None if top_logprobs is None else _vector(top_logprobs, dev, "torch.float32", (T, k),
+        lp = None if logprobs is None else _vector(logprobs, dev, _Types.f32, (T, G), f"{what}: logprobs")
+        ep = None if entropy is None else _vector(entropy, dev, _Types.f32, (T,), f"{what}: entropy")
+        ip = None if top_ids is None else _vector(top_ids, dev, _Types.i32, (T, k), f"{what}: top_ids")
+        bp = None if top_logprobs is None else _vector(top_logprobs, dev, _Types.f32, (T, k),
                                                        f"{what}: top_logprobs")
         return tp, G, k, lp, ep, ip, bp
 

@@ -30,6 +30,7 @@ def _context():
     c = object.__new__(har_cuda.Context)
     c.lib, c.handle, c.device = har_cuda.load_library(), None, 0
     c.last_error = lambda: ""
+    har_cuda._Types.load()
     return c
 
 
