@@ -69,14 +69,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     for (int w = 1; w < WARPS; ++w) top = max(top, part[threadIdx.x / TPR * WARPS + w]);
   }
   if (!live) return;
-  const bool finite = top < 0x7f800000u;
-  const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fffffff);
-  if (tid == 0) scale[row] = s;
-  const bool zero = !finite || s == 0.0f;
-  // x * (1/s) is within 2e-5 of the quotient, so it rounds to the same integer
-  // unless it lies that close to a half; only then is the quotient formed.
-  const bool exact = s < 1.17549435e-38f;  // 1/s may overflow
-  const float inv = exact || zero ? 0.0f : __fdiv_rn(1.0f, s);
+  const RowScale rs(top);
+  if (tid == 0) scale[row] = rs.s;
   int8_t *qr = q + row * ldq;
   auto put = [&](int64_t k0, const float (&u)[8]) {
     uint32_t w[2];
@@ -84,14 +78,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     for (int h = 0; h < 2; ++h) {
       uint32_t word = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = u[4 * h + i];
-        float t = __fmul_rn(a, inv);
-        float r = rintf(t);
-        if (exact || fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(a, s));
-        const int n = zero ? 0 : max(-127, min(127, (int)r));
-        word |= (uint32_t)(n & 0xff) << (8 * i);
-      }
+      for (int i = 0; i < 4; ++i) word |= (uint32_t)(rs.round(u[4 * h + i]) & 0xff) << (8 * i);
       w[h] = word;
     }
     if (q8 && k0 + 8 <= K) {

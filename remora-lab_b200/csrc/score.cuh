@@ -56,6 +56,29 @@ __device__ __forceinline__ unsigned long long order_key(float v, uint32_t id) {
   return ((unsigned long long)order_bits(v) << 32) | (0xffffffffu - id);
 }
 
+// The quantiser's rule for one row, from the largest |x| as bits (infinities
+// and NaN order above every number): s = max|x| / 127, q = rint(x / s), both
+// quotients rounded to f32.  x * (1/s) is within 2e-5 of the quotient, so it
+// rounds to the same integer unless it lies that close to a half; only then
+// (and where 1/s may overflow) is the quotient formed.
+struct RowScale {
+  float s, inv;
+  bool zero, exact;
+  __device__ __forceinline__ explicit RowScale(uint32_t top) {
+    const bool finite = top < 0x7f800000u;
+    s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fffffff);
+    zero = !finite || s == 0.0f;
+    exact = s < 1.17549435e-38f;
+    inv = exact || zero ? 0.0f : __fdiv_rn(1.0f, s);
+  }
+  __device__ __forceinline__ int round(float v) const {
+    const float t = __fmul_rn(v, inv);
+    float r = rintf(t);
+    if (exact || fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(v, s));
+    return zero ? 0 : max(-127, min(127, (int)r));
+  }
+};
+
 // Calls f with a value of the element type that `dtype` names.
 template <typename F>
 auto with_dtype(int32_t dtype, F &&f) {
@@ -78,6 +101,11 @@ int32_t launch_i8_quantize(har_cuda_ctx *ctx, const void *x, int32_t dtype, int6
 int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q,
                          int64_t ldq, const float *scale, int64_t M, void *y, int32_t y_dtype,
                          int64_t ldy);
+// The product for a few rows: whether it takes these sizes, and the launch, from
+// float rows (sx null: quantised on the way) or from 8-bit rows with scales sx.
+bool i8_gemv_takes(int64_t M, int64_t N, int64_t K);
+int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype,
+                       int64_t ldx, const float *sx, int64_t M, void *y, int32_t y_dtype, int64_t ldy);
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
                               int64_t V, int64_t ldl, const LogprobOut &out);
 
