@@ -1,0 +1,223 @@
+// i8_mma.cuh — the tensor-core pipeline that the 8-bit kernels share: TMA
+// producers, the MMA issuer, and the barriers between them and an epilogue.
+//
+//   D[A rows][B rows] = A [rows][K] * B [rows][K]^T, 32-bit sums in TMEM.
+//
+// CG = 1: a block computes tiles of 128 A rows x bn B rows.  CG = 2: a cluster
+// of two computes tiles of 256 x bn; each block loads its own 128 rows of A and
+// half the rows of B, so a k-step of 128 bytes brings 32 KB into a block's
+// shared memory for the same products that cost a lone block 48 KB.  Shared
+// memory moves 128 bytes a cycle and every byte crosses it twice (in by TMA,
+// out to the tensor core): a lone block at bn = 256 needs 750 cycles for 512
+// cycles of MMAs, a pair 512 for 512.
+#pragma once
+
+#include "score.cuh"
+#include "tc_ptx.cuh"
+
+namespace har {
+
+constexpr int G_A = 128, G_KS = 128, G_MAX_BN = 256;
+constexpr int G_STAGE_BYTES = 192 * 1024, G_MAX_STAGES = 12;
+constexpr int G_WARP_A = 0, G_WARP_MMA = 1, G_WARP_B = 2, G_WARP_EPI = 3, G_EPI_WARPS = 8;
+constexpr int G_EPI_THREADS = 32 * G_EPI_WARPS;
+constexpr int G_THREADS = 32 * G_WARP_EPI + G_EPI_THREADS;
+constexpr uint32_t G_WAIT_LIMIT = 1u << 22;
+
+struct Ring {
+  uint64_t full[G_MAX_STAGES], empty[G_MAX_STAGES], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// What every role knows: K in k-steps, the tile's columns, ring slots.
+struct RingShape {
+  int64_t K;
+  int bn, stages;
+  __device__ __forceinline__ int ksteps() const { return (int)((K + G_KS - 1) / G_KS); }
+};
+
+__device__ __forceinline__ bool g_wait(uint64_t *bar, uint32_t parity, volatile int *abort_s, uint32_t sleep_ns = 0) {
+  if (*abort_s) return false;
+  if (sleep_ns ? tc::mbar_wait_lazy(bar, parity, G_WAIT_LIMIT, sleep_ns) : tc::mbar_wait(bar, parity, G_WAIT_LIMIT))
+    return true;
+  *abort_s = 1;
+  return false;
+}
+__device__ __forceinline__ bool g_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_s, int lane,
+                                            uint32_t sleep_ns = 0) {
+  if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity))) return true;
+  bool ok = true;
+  if (lane == 0) ok = g_wait(bar, parity, abort_s, sleep_ns);
+  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+
+template <int CG>
+__device__ __forceinline__ void ring_open(Ring &r, const RingShape &sh, const void *map_a, const void *map_b) {
+  const int tid = threadIdx.x;
+  if (tid < 32) {
+    if (CG == 2) {
+      tc::tmem_alloc_pair(&r.tmem, 512);
+      tc::tmem_relinquish_pair();
+    } else {
+      tc::tmem_alloc(&r.tmem, 512);
+      tc::tmem_relinquish();
+    }
+  }
+  if (tid == 32) {
+    for (int s = 0; s < sh.stages; ++s) {
+      tc::mbar_init(r.full + s, 2);  // both producers
+      tc::mbar_init(r.empty + s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      tc::mbar_init(r.acc_full + a, 1);
+      tc::mbar_init(r.acc_empty + a, CG * G_EPI_WARPS);
+    }
+    tc::fence_mbar_init();
+    r.abort_flag = 0;
+  }
+  if (tid == 64) {
+    tc::tma_prefetch_desc(map_a);
+    tc::tma_prefetch_desc(map_b);
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (CG == 2) {  // the peer's barriers are initialised before anything arrives on them
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
+  tc::tc_fence_after();
+}
+
+template <int CG>
+__device__ __forceinline__ void ring_close(Ring &r, int *status) {
+  // a producer's lane rejoins its warp before the warp-wide instructions below
+  __syncwarp();
+  __syncthreads();
+  if (*(volatile int *)&r.abort_flag) {
+    if (threadIdx.x == 0) atomicOr(status, DEV_ERR_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // let copies and MMAs in flight land
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (CG == 2) {  // neither block leaves while the other's MMAs or arrivals may reach it
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
+  tc::tc_fence_after();
+  if (threadIdx.x < 32) {
+    __syncwarp();
+    if (CG == 2) tc::tmem_dealloc_pair(r.tmem, 512);
+    else tc::tmem_dealloc(r.tmem, 512);
+  }
+}
+
+// One lane loads the A boxes, a lane of another warp the B boxes, of the tiles
+// that `tiles` names: tiles.next(a_row, b_row).
+template <int CG, typename Tiles>
+__device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8_t *sm, bool is_b, const void *map,
+                                             Tiles tiles, uint32_t rank) {
+  volatile int *abort_s = &r.abort_flag;
+  const int b_rows = sh.bn / CG, ksteps = sh.ksteps();
+  const uint32_t a_bytes = G_A * G_KS, b_bytes = (uint32_t)b_rows * G_KS, bytes = is_b ? b_bytes : a_bytes;
+  uint32_t it = 0;
+  int a_row, b_row;
+  while (tiles.next(a_row, b_row)) {
+    const int row = is_b ? b_row + (int)rank * b_rows : a_row + (int)rank * G_A;
+    for (int k = 0; k < ksteps; ++k, ++it) {
+      const int s = (int)(it % (uint32_t)sh.stages);
+      if (!g_wait(r.empty + s, ((it / (uint32_t)sh.stages) & 1u) ^ 1u, abort_s, 64)) return;
+      uint8_t *dst = sm + (size_t)s * (a_bytes + b_bytes) + (is_b ? a_bytes : 0);
+      if (rank == 0) tc::mbar_expect_tx(r.full + s, CG * bytes);
+      if (CG == 2) tc::tma_load_2d_pair(dst, map, k * G_KS, row, tc::map_rank(tc::smem_u32(r.full + s), 0));
+      else tc::tma_load_2d(dst, map, k * G_KS, row, r.full + s);
+    }
+  }
+}
+
+// The MMA issuer: a whole warp (of the even block of a pair).
+template <int CG, typename Tiles>
+__device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t *sm, Tiles tiles) {
+  volatile int *abort_s = &r.abort_flag;
+  const int lane = threadIdx.x & 31, ksteps = sh.ksteps();
+  const uint32_t lead = tc::elect_one(), tmem = r.tmem;
+  const uint32_t a_bytes = G_A * G_KS, slot = a_bytes + (uint32_t)(sh.bn / CG) * G_KS;
+  const uint32_t idesc = tc::idesc_i8(CG * G_A, sh.bn);
+  const int last = (int)((sh.K - (int64_t)(ksteps - 1) * G_KS + 31) / 32);  // MMAs of the last k-step
+  uint32_t it = 0;
+  int a_row, b_row;
+  for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
+    const uint32_t a = n & 1u, par = ((n >> 1) & 1u) ^ 1u;
+    if (CG == 2) {  // arrivals of both blocks
+      bool ok = true;
+      if (lane == 0) {
+        ok = false;
+        for (uint32_t i = 0; i < G_WAIT_LIMIT && !ok && !*abort_s; ++i) ok = tc::mbar_try_wait_cluster(r.acc_empty + a, par);
+        if (!ok) *abort_s = 1;
+      }
+      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) return;
+    } else if (!g_wait_warp(r.acc_empty + a, par, abort_s, lane)) {
+      return;
+    }
+    tc::tc_fence_after();
+    const uint32_t d = tmem + a * 256u;
+    for (int k = 0; k < ksteps; ++k, ++it) {
+      const int s = (int)(it % (uint32_t)sh.stages);
+      if (!g_wait_warp(r.full + s, (it / (uint32_t)sh.stages) & 1u, abort_s, lane)) return;
+      tc::tc_fence_after();
+      const uint32_t base = tc::smem_u32(sm + (size_t)s * slot);
+      const uint64_t ad = tc::desc_sw128(base), bd = tc::desc_sw128(base + a_bytes);
+      const int slices = k == ksteps - 1 ? last : 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < slices) {
+          if (CG == 2) tc::mma_i8_pair_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, (k | j) ? 1u : 0u);
+          else tc::mma_i8_ss_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, (k | j) ? 1u : 0u);
+        }
+      if (CG == 2) tc::mma_commit_pair_w(lead, r.empty + s);
+      else tc::mma_commit_w(lead, r.empty + s);
+    }
+    if (CG == 2) tc::mma_commit_pair_w(lead, r.acc_full + a);
+    else tc::mma_commit_w(lead, r.acc_full + a);
+  }
+}
+
+// An epilogue warp is done reading accumulator a.
+template <int CG>
+__device__ __forceinline__ void ring_release(Ring &r, uint32_t a, int lane) {
+  tc::tc_fence_before();
+  __syncwarp();
+  if (lane == 0) {
+    if (CG == 2) tc::mbar_arrive_cluster(tc::map_rank(tc::smem_u32(r.acc_empty + a), 0));
+    else tc::mbar_arrive(r.acc_empty + a);
+  }
+}
+
+// Ring slots for tiles of bn columns.
+template <int CG>
+inline int ring_stages(int bn) {
+  const int slot = G_A * G_KS + bn / CG * G_KS, n = G_STAGE_BYTES / slot;
+  return n < G_MAX_STAGES ? n : G_MAX_STAGES;
+}
+
+// Launch of a kernel whose blocks work in clusters of `cluster`.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_clusters(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                            unsigned cluster, Args... args) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+}  // namespace har
