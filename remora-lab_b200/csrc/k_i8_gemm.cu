@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     i8_gemm_kernel(const __grid_constant__ TmaDesc map_w, const __grid_constant__ TmaDesc map_x, const GemmParams p) {
   extern __shared__ uint8_t g_raw[];
   __shared__ Ring ring;
+  __shared__ __align__(16) float scales[G_EPI_WARPS][G_MAX_BN / 2];
   uint8_t *sm = g_raw + ((1024u - (tc::smem_u32(g_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? tc::cluster_rank() : 0u;
@@ -64,10 +65,13 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     if (rank == 0) ring_issue<CG>(ring, p.sh, sm, GemmTiles<CG>(p));
   } else {
     // epilogue: lanes of quadrant warp % 4 are 32 channels; the two warps of a
-    // quadrant take the tile's 16-token chunks in turn
+    // quadrant take the tile's 16-token chunks in turn.  The tokens' scales wait
+    // in shared memory (a broadcast read each four), the next chunk's sums are
+    // on their way from tensor memory while this one's are written.
     volatile int *abort_s = &ring.abort_flag;
     const int g = warp & 3, h = (warp - G_WARP_EPI) >> 2;
     const uint32_t col0 = ring.tmem + ((uint32_t)(32 * g) << 16);
+    float *sx = scales[warp - G_WARP_EPI];
     GemmTiles<CG> tiles(p);
     int a_row, b_row;
     for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
@@ -77,18 +81,34 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       const float sw = live ? __ldg(p.sw + chan) : 0.0f;
       T *y = (T *)p.y + m0 * p.ldy + chan;
       const int rows = (int)min((int64_t)p.sh.bn, p.M - m0);
+#pragma unroll
+      for (int i = 0; i < G_MAX_BN / 64; ++i) {  // slot 32 i + lane: token 16 h + 64 i + (lane, chunks of 16 in turn)
+        const int c = 64 * i + 32 * (lane >> 4) + 16 * h + (lane & 15);
+        sx[32 * i + lane] = c < rows ? __ldg(p.sx + m0 + c) : 0.0f;
+      }
+      __syncwarp();
       if (!g_wait_warp(ring.acc_full + a, (n >> 1) & 1u, abort_s, lane)) break;
       tc::tc_fence_after();
-      for (int c = 16 * h; c < rows; c += 32) {
-        uint32_t v[16];
-        tc::tmem_ld16(col0 + a * 256u + (uint32_t)c, v);
-        const float sl = c + (lane & 15) < rows ? __ldg(p.sx + m0 + c + (lane & 15)) : 0.0f;
-        tc::tmem_wait_ld();
+      const uint32_t col = col0 + a * 256u;
+      uint32_t v[2][16];
+      if (16 * h < rows) tc::tmem_ld16(col + (uint32_t)(16 * h), v[0]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float s = __shfl_sync(0xffffffffu, sl, i);
-          if (live && c + i < rows)
-            y[(int64_t)(c + i) * p.ldy] = from_f32<T>(__fmul_rn(__int2float_rn((int)v[i]), __fmul_rn(s, sw)));
+      for (int j = 0; j < G_MAX_BN / 32; ++j) {
+        const int c = 16 * h + 32 * j;
+        if (c >= rows) break;
+        tc::tmem_wait_ld16(v[j & 1]);
+        if (c + 32 < rows) tc::tmem_ld16(col + (uint32_t)(c + 32), v[(j + 1) & 1]);
+        const float4 *s4 = reinterpret_cast<const float4 *>(sx + 16 * j);
+        T *yc = y + (int64_t)c * p.ldy;
+        const int here = live ? rows - c : 0;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 s = s4[i >> 2];
+          const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u < here)
+              yc[(i + u) * p.ldy] = from_f32<T>(__fmul_rn(__int2float_rn((int)v[j & 1][i + u]), __fmul_rn(f[u], sw)));
         }
       }
       ring_release<CG>(ring, a, lane);

@@ -29,8 +29,8 @@ __device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
 // rounding; longer rows are read again.
 template <typename T, int TPR, bool VEC>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
-    i8_quantize_kernel(const T *__restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                       int8_t *__restrict__ q, int64_t ldq, float *__restrict__ scale, int q8) {
+    i8_quantize_kernel(const T *__restrict__ x, int64_t M, int K, int64_t ldx, int8_t *__restrict__ q, int64_t ldq,
+                       float *__restrict__ scale, int q8) {
   constexpr int THREADS = TPR < 256 ? 256 : TPR;
   constexpr int ROWS = THREADS / TPR, HELD = 4;
   __shared__ uint32_t part[THREADS / 32];
@@ -39,27 +39,29 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
   const bool live = row < M;
   const T *xr = x + (live ? row : 0) * ldx;
   float v[HELD][8];
-  uint32_t top = 0;  // largest |x| as bits: infinities and NaN order above every number
+  float most = 0.0f;
 #pragma unroll
   for (int c = 0; c < HELD; ++c) {
-    const int64_t k0 = (int64_t)(c * TPR + tid) * 8;
-    const int n = live && k0 < K ? (int)(K - k0 < 8 ? K - k0 : 8) : 0;
-    if (n) {
+    const int k0 = (c * TPR + tid) * 8;
+    const int n = live ? min(8, K - k0) : 0;
+    if (n > 0) {
       load8<T, VEC>(xr + k0, n, v[c]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[c][i] = 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
   }
+#pragma unroll
+  for (int c = 0; c < HELD; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(v[c][i]));
   for (int64_t k0 = (int64_t)(HELD * TPR + tid) * 8; live && k0 < K; k0 += TPR * 8) {
     float u[8];
-    load8<T, VEC>(xr + k0, (int)(K - k0 < 8 ? K - k0 : 8), u);
+    load8<T, VEC>(xr + k0, min(8, K - (int)k0), u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(u[i]));
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
   if (TPR > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = top;
     __syncthreads();
@@ -73,30 +75,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
   if (tid == 0) scale[row] = rs.s;
   int8_t *qr = q + row * ldq;
   auto put = [&](int64_t k0, const float (&u)[8]) {
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t word = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) word |= (uint32_t)(rs.round(u[4 * h + i]) & 0xff) << (8 * i);
-      w[h] = word;
-    }
+    const uint2 w = make_uint2(rs.round4(u), rs.round4(u + 4));
     if (q8 && k0 + 8 <= K) {
-      *reinterpret_cast<uint2 *>(qr + k0) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2 *>(qr + k0) = w;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (k0 + i < K) qr[k0 + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
+        if (k0 + i < K) qr[k0 + i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
     }
   };
 #pragma unroll
   for (int c = 0; c < HELD; ++c) {
-    const int64_t k0 = (int64_t)(c * TPR + tid) * 8;
+    const int k0 = (c * TPR + tid) * 8;
     if (k0 < K) put(k0, v[c]);
   }
   for (int64_t k0 = (int64_t)(HELD * TPR + tid) * 8; k0 < K; k0 += TPR * 8) {
     float u[8];
-    load8<T, VEC>(xr + k0, (int)(K - k0 < 8 ? K - k0 : 8), u);
+    load8<T, VEC>(xr + k0, min(8, K - (int)k0), u);
     put(k0, u);
   }
 }
@@ -107,9 +102,9 @@ static void quantize_rows(har_cuda_ctx *ctx, const void *x, bool vec, int64_t M,
   constexpr int THREADS = TPR < 256 ? 256 : TPR;
   const unsigned grid = (unsigned)((M + THREADS / TPR - 1) / (THREADS / TPR));
   if (vec)
-    i8_quantize_kernel<T, TPR, true><<<grid, THREADS, 0, ctx->stream>>>((const T *)x, M, K, ldx, q, ldq, scale, q8);
+    i8_quantize_kernel<T, TPR, true><<<grid, THREADS, 0, ctx->stream>>>((const T *)x, M, (int)K, ldx, q, ldq, scale, q8);
   else
-    i8_quantize_kernel<T, TPR, false><<<grid, THREADS, 0, ctx->stream>>>((const T *)x, M, K, ldx, q, ldq, scale, q8);
+    i8_quantize_kernel<T, TPR, false><<<grid, THREADS, 0, ctx->stream>>>((const T *)x, M, (int)K, ldx, q, ldq, scale, q8);
 }
 
 int32_t launch_i8_quantize(har_cuda_ctx *ctx, const void *x, int32_t dtype, int64_t M, int64_t K,

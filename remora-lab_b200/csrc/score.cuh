@@ -56,12 +56,21 @@ __device__ __forceinline__ unsigned long long order_key(float v, uint32_t id) {
   return ((unsigned long long)order_bits(v) << 32) | (0xffffffffu - id);
 }
 
+// max that keeps a NaN of either side
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The quantiser's rule for one row, from the largest |x| as bits (infinities
 // and NaN order above every number): s = max|x| / 127, q = rint(x / s), both
-// quotients rounded to f32.  x * (1/s) is within 2e-5 of the quotient, so it
-// rounds to the same integer unless it lies that close to a half; only then
+// quotients rounded to f32.  Adding 1.5 * 2^23 to x * (1/s) leaves its nearest
+// integer in the low bits.  x * (1/s) is within 2e-5 of the quotient, so that
+// integer is the quotient's too unless it lies that close to a half; only then
 // (and where 1/s may overflow) is the quotient formed.
 struct RowScale {
+  static constexpr float MAGIC = 12582912.0f;
   float s, inv;
   bool zero, exact;
   __device__ __forceinline__ explicit RowScale(uint32_t top) {
@@ -71,11 +80,24 @@ struct RowScale {
     exact = s < 1.17549435e-38f;
     inv = exact || zero ? 0.0f : __fdiv_rn(1.0f, s);
   }
-  __device__ __forceinline__ int round(float v) const {
-    const float t = __fmul_rn(v, inv);
-    float r = rintf(t);
-    if (exact || fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(v, s));
-    return zero ? 0 : max(-127, min(127, (int)r));
+  __device__ __forceinline__ int slow(float v) const {
+    return zero ? 0 : max(-127, min(127, (int)rintf(__fdiv_rn(v, s))));
+  }
+  // four values as the bytes of a word
+  __device__ __forceinline__ uint32_t round4(const float *v) const {
+    const float2 i2 = make_float2(inv, inv), magic = make_float2(MAGIC, MAGIC), back = make_float2(-MAGIC, -MAGIC);
+    const float2 a = make_float2(v[0], v[1]), c = make_float2(v[2], v[3]);
+    const float2 ua = __ffma2_rn(a, i2, magic), uc = __ffma2_rn(c, i2, magic);
+    const float2 ra = __fadd2_rn(ua, back), rc = __fadd2_rn(uc, back);
+    const float2 da = __ffma2_rn(a, i2, make_float2(-ra.x, -ra.y)), dc = __ffma2_rn(c, i2, make_float2(-rc.x, -rc.y));
+    const float far = fmaxf(fmaxf(fabsf(da.x), fabsf(da.y)), fmaxf(fabsf(dc.x), fabsf(dc.y)));
+    if (exact || far > 0.4999f)
+      return (uint32_t)(slow(v[0]) & 0xff) | (uint32_t)(slow(v[1]) & 0xff) << 8 | (uint32_t)(slow(v[2]) & 0xff) << 16 |
+             (uint32_t)(slow(v[3]) & 0xff) << 24;
+    if (zero) return 0u;
+    const uint32_t lo = __byte_perm(__float_as_uint(ua.x), __float_as_uint(ua.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(uc.x), __float_as_uint(uc.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
   }
 };
 
@@ -103,7 +125,7 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
                          int64_t ldy);
 // The product for a few rows: whether it takes these sizes, and the launch, from
 // float rows (sx null: quantised on the way) or from 8-bit rows with scales sx.
-bool i8_gemv_takes(int64_t M, int64_t N, int64_t K);
+bool i8_gemv_takes(int64_t M, int64_t K);
 int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype,
                        int64_t ldx, const float *sx, int64_t M, void *y, int32_t y_dtype, int64_t ldy);
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
