@@ -18,7 +18,7 @@
 namespace har {
 
 constexpr int G_A = 128, G_KS = 128, G_MAX_BN = 256;
-constexpr int G_STAGE_BYTES = 192 * 1024, G_MAX_STAGES = 12;
+constexpr int G_STAGE_BYTES = 160 * 1024, G_MAX_STAGES = 12;
 constexpr int G_WARP_A = 0, G_WARP_MMA = 1, G_WARP_B = 2, G_WARP_EPI = 3, G_EPI_WARPS = 8;
 constexpr int G_EPI_THREADS = 32 * G_EPI_WARPS;
 constexpr int G_THREADS = 32 * G_WARP_EPI + G_EPI_THREADS;

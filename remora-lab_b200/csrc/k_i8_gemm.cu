@@ -11,12 +11,15 @@ namespace har {
 // then writes 32 neighbouring channels of one token with one store, and any
 // number of tokens from 1 up is one rule.
 constexpr int G_GROUP = 1024;  // channels swept together over all token tiles
+constexpr int G_SLAB = 8192;   // bytes of finished output on their way to memory
+constexpr int G_SLABS = 4;     // two for each half of the epilogue
 
 struct GemmParams {
   RingShape sh;
   int64_t M, N, ldy;
   const float *sx, *sw;
   void *y;
+  int store;          // y's rows take TMA stores
   int mt, nt;         // token and weight tiles
   int *status;
 };
@@ -46,11 +49,82 @@ struct GemmTiles {
   }
 };
 
+// One token's channels from shared memory to unaligned memory, a warp: whole
+// 4-byte words, a 2-byte type's odd first and last element apart.
+template <typename T>
+__device__ __forceinline__ void put_row(T *y, const T *row, int n, int lane) {
+  if (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < G_A; i += 32)
+      if (i + lane < n) y[i + lane] = row[i + lane];
+  } else {
+    const int odd = (int)((uintptr_t)y >> 1) & 1;
+    if (odd && n > 0 && lane == 0) y[0] = row[0];
+#pragma unroll
+    for (int i = 0; i < G_A; i += 64) {
+      const int e = odd + i + 2 * lane;
+      if (e + 1 < n) {
+        const T two[2] = {row[e], row[e + 1]};
+        *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(two);
+      } else if (e < n) {
+        y[e] = row[e];
+      }
+    }
+  }
+}
+
+// Output of `n` tokens (at most 128, from token m) of 128 channels, by the
+// four warps of one half; v holds this thread's channel.  Finished values are
+// laid out in shared memory, [token][128 channels], and written by TMA, or row
+// by row where y's rows do not start at multiples of 16 bytes: a 2-byte value a
+// lane straight to memory took 12,600 cycles a tile, against 12,000 of MMAs at
+// K = 2048, and held them up.
+template <typename T>
+__device__ __forceinline__ void put_slabs(const GemmParams &p, const void *map_y, uint8_t *slabs, const float *sx, float sw,
+                                          uint32_t (&v)[4][32], int n, int64_t m, int chan0, int h, int quad, int lane,
+                                          uint32_t &used) {
+  constexpr int TOK = G_SLAB / (G_A * (int)sizeof(T));  // tokens of a slab: 32, or 16 of f32
+  const int id = 1 + h;
+#pragma unroll
+  for (int i = 0; i < 128 / TOK; ++i, ++used) {
+    if (i * TOK >= n) break;
+    T *slab = reinterpret_cast<T *>(slabs + (2 * h + (used & 1u)) * G_SLAB);
+    if (p.store && quad == 0 && lane == 0) tc::bulk_wait_read<1>();  // the slab two before has been read
+    tc::bar_sync(id, 128);
+#pragma unroll
+    for (int t = 0; t < TOK; t += 4) {
+      const int c = i * TOK + t;
+      const float4 s = *reinterpret_cast<const float4 *>(sx + c);
+      const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        slab[(t + u) * G_A + 32 * quad + lane] =
+            from_f32<T>(__fmul_rn(__int2float_rn((int)v[(c + u) >> 5][(c + u) & 31]), __fmul_rn(f[u], sw)));
+    }
+    if (p.store) tc::fence_proxy_async_smem();
+    tc::bar_sync(id, 128);
+    if (p.store) {
+      if (quad == 0 && lane == 0) {
+#pragma unroll
+        for (int t = 0; t < TOK; t += 16)
+          if (i * TOK + t < n && chan0 < p.N) tc::tma_store_2d(map_y, chan0, (int)m + i * TOK + t, slab + t * G_A);
+        tc::bulk_commit();
+      }
+    } else {
+      T *y = (T *)p.y + (m + i * TOK) * p.ldy + chan0;
+      const int chans = (int)min((int64_t)G_A, p.N - chan0);
+      for (int t = quad; t < min(TOK, n - i * TOK); t += 4) put_row(y + t * p.ldy, slab + t * G_A, chans, lane);
+    }
+  }
+}
+
 template <typename T, int CG>
 __global__ void __launch_bounds__(G_THREADS, 1)
-    i8_gemm_kernel(const __grid_constant__ TmaDesc map_w, const __grid_constant__ TmaDesc map_x, const GemmParams p) {
+    i8_gemm_kernel(const __grid_constant__ TmaDesc map_w, const __grid_constant__ TmaDesc map_x,
+                   const __grid_constant__ TmaDesc map_y, const GemmParams p) {
   extern __shared__ uint8_t g_raw[];
   __shared__ Ring ring;
+  __shared__ int go[2][2];
   __shared__ __align__(16) float scales[G_EPI_WARPS][G_MAX_BN / 2];
   uint8_t *sm = g_raw + ((1024u - (tc::smem_u32(g_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -64,65 +138,62 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   } else if (warp == G_WARP_MMA) {
     if (rank == 0) ring_issue<CG>(ring, p.sh, sm, GemmTiles<CG>(p));
   } else {
-    // epilogue: lanes of quadrant warp % 4 are 32 channels; the two warps of a
-    // quadrant take the tile's 16-token chunks in turn.  The tokens' scales wait
-    // in shared memory (a broadcast read each four), the next chunk's sums are
-    // on their way from tensor memory while this one's are written.
+    // epilogue: lanes of quadrant warp % 4 are 32 channels, half h of the warps
+    // takes half of the tile's tokens: it reads its sums into registers in one
+    // go, gives the accumulator back and only then converts and writes
     volatile int *abort_s = &ring.abort_flag;
-    const int g = warp & 3, h = (warp - G_WARP_EPI) >> 2;
-    const uint32_t col0 = ring.tmem + ((uint32_t)(32 * g) << 16);
+    const int quad = warp & 3, h = (warp - G_WARP_EPI) >> 2;
+    const uint32_t col0 = ring.tmem + ((uint32_t)(32 * quad) << 16);
+    const int half = (p.sh.bn / 16 + 1) / 2 * 16;
     float *sx = scales[warp - G_WARP_EPI];
+    uint8_t *slabs = sm + G_STAGE_BYTES;
+    uint32_t used = 0;  // slabs written so far
     GemmTiles<CG> tiles(p);
     int a_row, b_row;
     for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
       const uint32_t a = n & 1u;
-      const int64_t chan = (int64_t)a_row + rank * G_A + 32 * g + lane, m0 = b_row;
+      const int chan0 = a_row + (int)rank * G_A;
+      const int64_t chan = (int64_t)chan0 + 32 * quad + lane, m = (int64_t)b_row + h * half;
       const bool live = chan < p.N;
       const float sw = live ? __ldg(p.sw + chan) : 0.0f;
-      T *y = (T *)p.y + m0 * p.ldy + chan;
-      const int rows = (int)min((int64_t)p.sh.bn, p.M - m0);
+      // this half's tokens: within the tile, and within M
+      const int mine = (int)max((int64_t)0, min((int64_t)(h == 0 ? half : p.sh.bn - half), p.M - m));
 #pragma unroll
-      for (int i = 0; i < G_MAX_BN / 64; ++i) {  // slot 32 i + lane: token 16 h + 64 i + (lane, chunks of 16 in turn)
-        const int c = 64 * i + 32 * (lane >> 4) + 16 * h + (lane & 15);
-        sx[32 * i + lane] = c < rows ? __ldg(p.sx + m0 + c) : 0.0f;
+      for (int i = 0; i < G_MAX_BN / 64; ++i) {
+        const int c = 32 * i + lane;
+        sx[c] = c < mine ? __ldg(p.sx + m + c) : 0.0f;
       }
       __syncwarp();
-      if (!g_wait_warp(ring.acc_full + a, (n >> 1) & 1u, abort_s, lane)) break;
-      tc::tc_fence_after();
-      const uint32_t col = col0 + a * 256u;
-      uint32_t v[2][16];
-      if (16 * h < rows) tc::tmem_ld16(col + (uint32_t)(16 * h), v[0]);
-#pragma unroll
-      for (int j = 0; j < G_MAX_BN / 32; ++j) {
-        const int c = 16 * h + 32 * j;
-        if (c >= rows) break;
-        tc::tmem_wait_ld16(v[j & 1]);
-        if (c + 32 < rows) tc::tmem_ld16(col + (uint32_t)(c + 32), v[(j + 1) & 1]);
-        const float4 *s4 = reinterpret_cast<const float4 *>(sx + 16 * j);
-        T *yc = y + (int64_t)c * p.ldy;
-        const int here = live ? rows - c : 0;
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 s = s4[i >> 2];
-          const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (i + u < here)
-              yc[(i + u) * p.ldy] = from_f32<T>(__fmul_rn(__int2float_rn((int)v[j & 1][i + u]), __fmul_rn(f[u], sw)));
-        }
+      // one warp waits for the half and says whether to go on, so that all four
+      // leave together when a wait gave up
+      if (quad == 0) {
+        const bool ok = g_wait_warp(ring.acc_full + a, (n >> 1) & 1u, abort_s, lane, 256);
+        if (lane == 0) go[h][a] = ok;
       }
+      tc::bar_sync(1 + h, 128);
+      if (!go[h][a]) break;
+      tc::tc_fence_after();
+      const uint32_t col = col0 + a * 256u + (uint32_t)(h * half);
+      uint32_t v[4][32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (32 * j < mine) tc::tmem_ld32(col + (uint32_t)(32 * j), v[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tc::tmem_wait_ld32(v[j]);
       ring_release<CG>(ring, a, lane);
+      put_slabs<T>(p, &map_y, slabs, sx, sw, v, mine, m, chan0, h, quad, lane, used);
     }
+    if (p.store && quad == 0 && lane == 0) tc::bulk_wait<0>();
   }
   ring_close<CG>(ring, p.status);
 }
 
 // Blocks a tile and tokens of a tile: the split of M into equal tiles that
 // costs least.  A k-step of a tile costs a lone block its MMAs (2 cycles a
-// token at 8,192 products a cycle) or its bytes from L2 (about 64 a cycle) or
-// its bytes through shared memory, in and out (128 a cycle), whichever is most;
-// a pair moves half the token bytes.  A tile costs about 1,500 cycles to fill
-// and drain, a pair 500 more to join.
+// token at 8,192 products a cycle) or its bytes from L2 (about 42 a cycle
+// measured, with all blocks loading), whichever is more; a pair moves half the
+// token bytes.  A tile costs about 1,500 cycles to fill and drain, a pair 500
+// more to join.
 static int pick_tile(int64_t M, int64_t N, int64_t K, int sms, int &cg) {
   const int64_t ksteps = (K + G_KS - 1) / G_KS;
   double best = 0;
@@ -133,8 +204,7 @@ static int pick_tile(int64_t M, int64_t N, int64_t K, int sms, int &cg) {
       const int64_t b = ((M + mt - 1) / mt + 16 * g - 1) / (16 * g) * (16 * g);
       const int64_t tiles = nt * ((M + b - 1) / b), waves = (tiles + sms / g - 1) / (sms / g);
       const double bytes = G_A * G_KS + b / g * G_KS;
-      const double step = std::max({2.0 * b, bytes / 64.0});
-      const double cost = waves * (ksteps * std::max(step, 2.0 * bytes / 128.0) + 1500.0 + 500.0 * (g - 1));
+      const double cost = waves * (ksteps * std::max(2.0 * b, bytes / 42.0) + 1500.0 + 500.0 * (g - 1));
       if (!bn || cost < best) best = cost, bn = (int)b, cg = g;
     }
   }
@@ -156,14 +226,24 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
   TmaDesc map_x;
   int32_t st = encode_tmap_2d(ctx, &map_x, q, 1, (uint64_t)M, (uint64_t)w->K, (uint64_t)ldq, (uint32_t)(p.sh.bn / cg), G_KS, true);
   if (st != HAR_CUDA_OK) return st;
+  // y by TMA where its rows start and end at multiples of 16 bytes (a TMA
+  // store fills the last 16 bytes of a row with zeros)
+  TmaDesc map_y = map_x;
+  const size_t eb = dtype_bytes(y_dtype);
+  p.store = ((uintptr_t)y & 15u) == 0 && (w->N * (int64_t)eb) % 16 == 0 && (M == 1 || (ldy * (int64_t)eb) % 16 == 0);
+  if (p.store) {
+    const uint64_t pitch = (uint64_t)(M == 1 ? w->N : ldy) * eb;
+    st = encode_tmap_2d(ctx, &map_y, y, (int)eb, (uint64_t)M, (uint64_t)w->N, pitch, 16, G_A, false);
+    if (st != HAR_CUDA_OK) return st;
+  }
   const unsigned grid = (unsigned)std::min<int64_t>(ctx->num_sms / cg, (int64_t)p.mt * p.nt) * cg;
   cudaError_t e = cudaSuccess;
   prof_begin(ctx);
   with_dtype(y_dtype, [&](auto t) {
     using T = decltype(t);
-    const size_t smem = G_STAGE_BYTES + 1024;
-    e = cg == 2 ? launch_clusters(i8_gemm_kernel<T, 2>, grid, G_THREADS, smem, ctx->stream, 2, w->map, map_x, p)
-                : launch_clusters(i8_gemm_kernel<T, 1>, grid, G_THREADS, smem, ctx->stream, 1, w->map, map_x, p);
+    const size_t smem = G_STAGE_BYTES + G_SLABS * G_SLAB + 1024;
+    e = cg == 2 ? launch_clusters(i8_gemm_kernel<T, 2>, grid, G_THREADS, smem, ctx->stream, 2, w->map, map_x, map_y, p)
+                : launch_clusters(i8_gemm_kernel<T, 1>, grid, G_THREADS, smem, ctx->stream, 1, w->map, map_x, map_y, p);
   });
   st = check_launch(ctx, "i8_gemm_kernel");
   if (e != cudaSuccess)

@@ -39,7 +39,9 @@ int32_t encode_tmap_2d(har_cuda_ctx *ctx, TmaDesc *out, const void *base, int el
   if (((uintptr_t)base & 15u) || (row_stride & 15u))
     return set_error(ctx, HAR_CUDA_ERR_ARG, "tensor map: base and row stride must be 16-byte aligned");
   const CUtensorMapDataType dt =
-      elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+      : elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {row_stride};
   const cuuint32_t box[2] = {box_cols, box_rows};

@@ -109,6 +109,12 @@ def test_linear_and_matmul(ctx, M, N, K, ydtype):
     q, s = quantized(ctx, x)
     ctx.i8_matmul(w, q, s, y)
     assert torch.equal(y.cpu(), ref)
+    whole = torch.full((M + 2, (N + 23) // 8 * 8), 9.0, dtype=DT[ydtype], device="cuda")
+    z = whole[1:M + 1, 8:N + 8]                   # rows at multiples of 16 bytes
+    ctx.i8_matmul(w, q, s, z)
+    assert torch.equal(z.cpu(), ref)
+    assert (whole[0] == 9).all() and (whole[M + 1] == 9).all()
+    assert (whole[:, :8] == 9).all() and (whole[:, N + 8:] == 9).all()
     assert (buf[0] == 9).all() and (buf[M + 1] == 9).all()
     assert (buf[:, :2] == 9).all() and (buf[:, N + 2:] == 9).all()
 
