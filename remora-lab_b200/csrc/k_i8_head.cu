@@ -1,0 +1,540 @@
+// k_i8_head.cu — log probabilities straight from hidden states and an 8-bit LM
+// head: the product's epilogue folds every logit into its row's sums and keeps
+// the largest, so the [T][V] logits are never stored (f32 logits of 2,048
+// tokens x 131,072 would be 1 GB written and 1 GB read back).
+#include <algorithm>
+
+#include "i8_mma.cuh"
+#include "logprob_row.cuh"
+
+namespace har {
+
+// A block's tile is 128 tokens (tensor-memory lanes) x 128 CG vocabulary rows
+// (columns): a thread of the epilogue owns one token and half the columns, and
+// keeps the token's sums and list to itself.
+constexpr int H_CAP = 96;          // entries of a thread's list: 64, and 32 of the columns in hand
+constexpr int H_FULL = H_CAP - 32;
+constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
+constexpr int64_t H_TOKENS = 4096; // tokens of one launch
+
+struct HeadPlan {
+  int cg, tt, vt, g, C, passes;    // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
+  int64_t Tp;                      // tokens rounded up to tiles
+  int parts() const { return 2 * C; }
+  int blocks() const { return g * C * cg; }
+};
+
+struct HeadParams {
+  RingShape sh;
+  int64_t T, V, Tp;
+  const float *sx, *sw;
+  int tt, vt, g, C, k;
+  float *list_v;                   // [block][H_CAP][256]: the threads' working lists
+  int32_t *list_i;
+  // part 2 c + h (stream c, half h of a tile's columns) of token t at [part][t]
+  float *part_r, *part_s, *part_t;
+  key_t *part_best;                // its largest key, 0: no entry
+  int32_t *part_n;                 // its entries
+  float *part_v;                   // [part][k][Tp]
+  int32_t *part_i;
+  int *status;
+};
+
+// Block (or pair) b works on token tile pass * g + b / C and vocabulary tiles
+// b % C, b % C + C, ...: the g pairs of a stream read the same weights at about
+// the same time, so they come from memory once.
+template <int CG>
+struct HeadTiles {
+  const HeadParams &p;
+  int slot, c, pass, v;
+  __device__ __forceinline__ explicit HeadTiles(const HeadParams &p_) : p(p_), pass(0) {
+    const int b = blockIdx.x / CG;
+    slot = b / p.C;
+    c = v = b - slot * p.C;
+  }
+  __device__ __forceinline__ bool next(int &a_row, int &b_row) {
+    if (v >= p.vt) {
+      ++pass;
+      v = c;
+    }
+    const int t = pass * p.g + slot;
+    if (t >= p.tt) return false;
+    a_row = t * (CG * G_A);
+    b_row = v * (CG * G_A);
+    v += p.C;
+    return true;
+  }
+};
+
+// 32 values a thread in descending order (bitonic, in registers).
+__device__ __forceinline__ void sort32_desc(float (&v)[32]) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int step = size >> 1; step > 0; step >>= 1)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int j = i ^ step;
+        if (j > i) {
+          const float hi = fmaxf(v[i], v[j]), lo = fminf(v[i], v[j]);
+          const bool desc = (i & size) == 0;
+          v[i] = desc ? hi : lo;
+          v[j] = desc ? lo : hi;
+        }
+      }
+}
+// a <- the 32 largest of two descending runs.
+__device__ __forceinline__ void merge32_desc(float (&a)[32], const float (&b)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) a[i] = fmaxf(a[i], b[31 - i]);
+#pragma unroll
+  for (int step = 16; step > 0; step >>= 1)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int j = i ^ step;
+      if (j > i) {
+        const float hi = fmaxf(a[i], a[j]), lo = fminf(a[i], a[j]);
+        a[i] = hi;
+        a[j] = lo;
+      }
+    }
+}
+__device__ __forceinline__ float pick32(const float (&v)[32], int i) {
+  float r = v[0];
+#pragma unroll
+  for (int j = 1; j < 32; ++j) r = j == i ? v[j] : r;
+  return r;
+}
+
+struct ListState {
+  int n;
+  float bar;
+};
+// Cuts a thread's list back to its k largest entries: the k-th value from a
+// sort of the values alone, then one sweep that keeps what is above it and, of
+// its equals, the first (entries stand in the order of their ids).  The whole
+// warp; a thread with fewer than k entries keeps them and its bar.
+__device__ __noinline__ ListState list_cut(float *v, int32_t *id, ListState s, int k) {
+  float top[32], more[32];
+  const int most = __reduce_max_sync(0xffffffffu, s.n);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top[i] = i < s.n ? v[i * G_EPI_THREADS] : -INFINITY;
+  sort32_desc(top);
+  for (int b = 32; b < most; b += 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) more[i] = b + i < s.n ? v[(b + i) * G_EPI_THREADS] : -INFINITY;
+    sort32_desc(more);
+    merge32_desc(top, more);
+  }
+  if (s.n < k) return s;
+  const float bar = pick32(top, k - 1);
+  int equals = k;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) equals -= i < k && top[i] > bar;
+  int n = 0;
+  for (int e0 = 0; e0 < s.n; e0 += 8) {
+    float x[8];
+    int32_t y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = e0 + i < s.n ? v[(e0 + i) * G_EPI_THREADS] : -INFINITY;
+      y[i] = e0 + i < s.n ? id[(e0 + i) * G_EPI_THREADS] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool keep = e0 + i < s.n && (x[i] > bar || (x[i] == bar && equals-- > 0));
+      if (keep) {
+        v[n * G_EPI_THREADS] = x[i];
+        id[n * G_EPI_THREADS] = y[i];
+        ++n;
+      }
+    }
+  }
+  return {n, bar};
+}
+
+template <int CG>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    i8_head_kernel(const __grid_constant__ TmaDesc map_x, const __grid_constant__ TmaDesc map_w, const HeadParams p) {
+  constexpr int COLS = 64 * CG;  // a thread's columns of a tile
+  extern __shared__ uint8_t g_raw[];
+  __shared__ Ring ring;
+  __shared__ int go[2][2];
+  __shared__ __align__(16) float scales[2][2][COLS];
+  uint8_t *sm = g_raw + ((1024u - (tc::smem_u32(g_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? tc::cluster_rank() : 0u;
+  ring_open<CG>(ring, p.sh, &map_x, &map_w);
+
+  if (warp == G_WARP_A) {
+    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, false, &map_x, HeadTiles<CG>(p), rank);
+  } else if (warp == G_WARP_B) {
+    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, true, &map_w, HeadTiles<CG>(p), rank);
+  } else if (warp == G_WARP_MMA) {
+    if (rank == 0) ring_issue<CG>(ring, p.sh, sm, HeadTiles<CG>(p));
+  } else {
+    volatile int *abort_s = &ring.abort_flag;
+    const int quad = warp & 3, h = (warp - G_WARP_EPI) >> 2;
+    const int row = 32 * quad + lane, me = h * 128 + row;
+    const uint32_t col0 = ring.tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(h * COLS);
+    float *lv = p.list_v + (int64_t)blockIdx.x * (H_CAP * G_EPI_THREADS) + me;
+    int32_t *li = p.list_i + (int64_t)blockIdx.x * (H_CAP * G_EPI_THREADS) + me;
+    HeadTiles<CG> tiles(p);
+    Stat st = {-INFINITY, 0.0f, 0.0f};
+    ListState ls = {0, INFINITY};
+    int64_t token = -1;
+    float sx = 0.0f;
+    int cur = -1;
+
+    // the token tile's part is done
+    auto flush = [&]() {
+      if (p.k > 0) ls = list_cut(lv, li, ls, p.k);
+      if (token >= p.T) return;
+      const int64_t at = (int64_t)(2 * tiles.c + h) * p.Tp + token;
+      p.part_r[at] = st.r;
+      p.part_s[at] = st.s;
+      p.part_t[at] = st.t;
+      if (p.k == 0) return;
+      key_t best = 0;
+      for (int e = 0; e < ls.n; ++e) {
+        const float x = lv[e * G_EPI_THREADS];
+        const int32_t id = li[e * G_EPI_THREADS];
+        const int64_t to = ((int64_t)(2 * tiles.c + h) * p.k + e) * p.Tp + token;
+        p.part_v[to] = x;
+        p.part_i[to] = id;
+        best = key_max(best, order_key(x, (uint32_t)id));
+      }
+      p.part_n[at] = ls.n;
+      p.part_best[at] = best;
+    };
+
+    int a_row, b_row;
+    for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
+      const uint32_t a = n & 1u;
+      bool first = false;
+      if (a_row != cur) {
+        if (cur >= 0) flush();
+        cur = a_row;
+        first = true;
+        token = (int64_t)a_row + rank * G_A + row;
+        sx = token < p.T ? __ldg(p.sx + token) : 0.0f;
+        st = {-INFINITY, 0.0f, 0.0f};
+        ls = {0, token < p.T ? -INFINITY : INFINITY};
+      }
+      const int64_t v0 = (int64_t)b_row + h * COLS;  // this half's first vocabulary row
+      if (row < COLS) scales[a][h][row] = v0 + row < p.V ? __ldg(p.sw + v0 + row) : 0.0f;
+      if (quad == 0) {
+        const bool ok = g_wait_warp(ring.acc_full + a, (n >> 1) & 1u, abort_s, lane, 256);
+        if (lane == 0) go[h][a] = ok;
+      }
+      tc::bar_sync(1 + h, 128);
+      if (!go[h][a]) {
+        cur = -1;  // nothing to flush
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t col = col0 + a * 256u;
+      const bool ragged = v0 + COLS > p.V;
+      // 32 logits from column c on, as i8_linear writes them; -inf past V
+      auto logits = [&](int c, float (&l)[32]) {
+        uint32_t v[32];
+        tc::tmem_ld32(col + (uint32_t)c, v);
+        tc::tmem_wait_ld32(v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 s = *reinterpret_cast<const float4 *>(&scales[a][h][c + i]);
+          l[i] = __fmul_rn(__int2float_rn((int)v[i]), __fmul_rn(sx, s.x));
+          l[i + 1] = __fmul_rn(__int2float_rn((int)v[i + 1]), __fmul_rn(sx, s.y));
+          l[i + 2] = __fmul_rn(__int2float_rn((int)v[i + 2]), __fmul_rn(sx, s.z));
+          l[i + 3] = __fmul_rn(__int2float_rn((int)v[i + 3]), __fmul_rn(sx, s.w));
+        }
+        if (ragged) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) l[i] = v0 + c + i < p.V ? l[i] : -INFINITY;
+        }
+      };
+      if (first && p.k > 0) {
+        // the k-th largest of 32 groups' largest logits: k logits are at least
+        // as large, so the list starts behind a float below them
+        float top[32];
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          float l[32];
+          logits(c, l);
+          constexpr int W = COLS / 32;  // columns of a group
+#pragma unroll
+          for (int i = 0; i < 32; i += W) {
+            float m = l[i];
+#pragma unroll
+            for (int j = 1; j < W; ++j) m = fmaxf(m, l[i + j]);
+            top[(c + i) / W] = fmaxf(m, -INFINITY);
+          }
+        }
+        sort32_desc(top);
+        const uint32_t o = order_bits(pick32(top, p.k - 1));
+        // two steps down: the one below +0 is -0, its equal
+        if (token < p.T) ls.bar = order_value(max(o - 2u, order_bits(-INFINITY)));
+      }
+#pragma unroll
+      for (int c = 0; c < COLS; c += 32) {
+        float l[32];
+        logits(c, l);
+        if (c + 32 == COLS) ring_release<CG>(ring, a, lane);
+        float top = l[0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) top = fmaxf(top, l[i]);
+        if (p.k > 0 && __any_sync(0xffffffffu, top > ls.bar)) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (l[i] > ls.bar) {
+              lv[ls.n * G_EPI_THREADS] = l[i];
+              li[ls.n * G_EPI_THREADS] = (int32_t)(v0 + c + i);
+              ++ls.n;
+            }
+          if (__any_sync(0xffffffffu, ls.n > H_FULL)) ls = list_cut(lv, li, ls, p.k);
+        }
+        stat_add<32>(st, top, [&](int i) { return l[i]; });
+      }
+    }
+    if (cur >= 0) flush();
+  }
+  ring_close<CG>(ring, p.status);
+}
+
+// ---- joining the parts --------------------------------------------------------------
+
+struct HeadJoin {
+  HeadParams p;
+  LogprobOut out;
+  const int8_t *x, *w;   // quantised rows, for the given tokens' logits
+  int64_t ldx, ldw, K;
+  int parts;
+};
+
+// Exact dot product of two 8-bit rows by one warp.
+__device__ __forceinline__ int warp_dot(const int8_t *a, const int8_t *b, int64_t K, int lane) {
+  int acc = 0;
+  for (int64_t k = 16 * lane; k < K; k += 512) {
+    if (k + 16 <= K) {
+      const uint4 u = ldg_nc_v4(a + k), v = ldg_nc_v4(b + k);
+      acc = __dp4a((int)u.x, (int)v.x, acc);
+      acc = __dp4a((int)u.y, (int)v.y, acc);
+      acc = __dp4a((int)u.z, (int)v.z, acc);
+      acc = __dp4a((int)u.w, (int)v.w, acc);
+    } else {
+      for (int i = 0; k + i < K; ++i) acc += (int)a[k + i] * (int)b[k + i];
+    }
+  }
+  return __reduce_add_sync(0xffffffffu, acc);
+}
+
+// One block a token.  The alternatives are found as in the walk over logits: a
+// part whose largest key is below the k-th largest of the parts' has none, so
+// at most k parts, of at most k entries each, are read.
+template <int TH>
+__global__ void __launch_bounds__(TH) head_join_kernel(const HeadJoin j) {
+  constexpr int W = TH / 32, LISTS = W <= 2 ? 2 : 16;
+  __shared__ Stat stats[W];
+  __shared__ key_t lists[LISTS][32];
+  __shared__ key_t cand[I8_MAX_TOP * I8_MAX_TOP];
+  __shared__ key_t bound_s;
+  __shared__ int count;
+  const HeadParams &p = j.p;
+  const LogprobOut &out = j.out;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t t = blockIdx.x;
+  const float sx = p.sx[t];
+  Stat st = {-INFINITY, 0.0f, 0.0f};
+  if (tid < j.parts) {
+    const int64_t at = (int64_t)tid * p.Tp + t;
+    st = {p.part_r[at], p.part_s[at], p.part_t[at]};
+  }
+  st = warp_stat(st);
+  if (lane == 0) stats[warp] = st;
+  key_t best = p.k > 0 && tid < j.parts ? p.part_best[(int64_t)tid * p.Tp + t] : 0;
+  for (int i = tid; i < LISTS * 32; i += TH) (&lists[0][0])[i] = 0;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  st = warp_stat(lane < W ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+  const RowEnd end(st);
+  if (tid == 0 && out.entropy) out.entropy[t] = end.entropy;
+  if (out.logprobs)
+    for (int g = warp; g < out.G; g += W) {
+      const int32_t tok = out.tokens[t * out.G + g];
+      float r = 0.0f;
+      if (tok >= 0 && tok < p.V) {
+        const int acc = warp_dot(j.x + t * j.ldx, j.w + tok * j.ldw, j.K, lane);
+        r = end.logp(__fmul_rn(__int2float_rn(acc), __fmul_rn(sx, p.sw[tok])));
+      } else if (tok != -1) {
+        r = __int_as_float(0x7fffffff);
+        if (lane == 0) atomicOr(out.status, DEV_ERR_BOUNDS);
+      }
+      if (lane == 0) out.logprobs[t * out.G + g] = r;
+    }
+  if (p.k == 0) return;
+
+  lists[warp][lane] = warp_sort_desc(best, lane);
+  __syncthreads();
+  const key_t merged = block_merge_lists(lists, LISTS, warp, lane);
+  if (warp == 0 && lane == p.k - 1) bound_s = key_max(merged, (key_t)1);
+  __syncthreads();
+  const key_t bound = bound_s;
+  if (best >= bound) {
+    const int n = p.part_n[(int64_t)tid * p.Tp + t];
+    for (int e = 0; e < n; ++e) {
+      const int64_t at = ((int64_t)tid * p.k + e) * p.Tp + t;
+      const key_t key = order_key(p.part_v[at], (uint32_t)p.part_i[at]);
+      if (key >= bound) cand[atomicAdd(&count, 1)] = key;
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  key_t list = 0;
+  for (int i = 32 * warp; i < n; i += TH)
+    list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? cand[i + lane] : (key_t)0, lane), lane);
+  for (int i = W * 32 + tid; i < LISTS * 32; i += TH) (&lists[0][0])[i] = 0;
+  lists[warp][lane] = list;
+  __syncthreads();
+  best = block_merge_lists(lists, LISTS, warp, lane);
+  if (warp != 0) return;
+  int id = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
+  const float lp = best ? end.logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
+  // Places left go to -inf logits, then to NaN, each by id.  A logit is neither
+  // unless its scale is NaN, or so large that the product may overflow.
+  int have = __popc(__ballot_sync(0xffffffffu, best != 0));
+  for (int pass = sx == sx ? 0 : 1; pass < 2 && have < p.k; ++pass)
+    for (int64_t v = lane; have < p.k && v - lane < p.V; v += 32) {
+      const float s = v < p.V ? __fmul_rn(sx, p.sw[v]) : 0.0f;
+      uint32_t odd = __ballot_sync(0xffffffffu, !(fabsf(s) < 1e28f));
+      for (; odd && have < p.k; odd &= odd - 1) {
+        const int b = __ffs(odd) - 1;
+        const float sb = __shfl_sync(0xffffffffu, s, b);
+        const int64_t vb = v - lane + b;
+        float x = sb;
+        if (sb == sb) x = __fmul_rn(__int2float_rn(warp_dot(j.x + t * j.ldx, j.w + vb * j.ldw, j.K, lane)), sb);
+        if (pass == 0 ? x == -INFINITY : x != x) {
+          if (lane == have) id = (int)vb;
+          ++have;
+        }
+      }
+    }
+  if (lane < p.k) {
+    const int64_t o = t * p.k + lane;
+    if (out.top_ids) out.top_ids[o] = id;
+    if (out.top_logprobs) out.top_logprobs[o] = end.s != end.s ? end.s : lp;
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+// Pairs of blocks above 128 tokens.  Token tiles at a time: the number that
+// takes the fewest steps of a tile, more of them (fewer parts) for equal steps.
+static HeadPlan head_plan(int64_t T, int64_t V, int sms) {
+  HeadPlan h = {};
+  h.cg = T > G_A ? 2 : 1;
+  const int tile = G_A * h.cg, slots = sms / h.cg;
+  h.tt = (int)((T + tile - 1) / tile);
+  h.vt = (int)((V + tile - 1) / tile);
+  h.Tp = (int64_t)h.tt * tile;
+  double best = 0;
+  for (int g = std::min(h.tt, slots); g >= 1; --g) {
+    const int C = std::min({h.vt, slots / g, H_JOIN_MOST / 2}), passes = (h.tt + g - 1) / g;
+    const double cost = passes * ((h.vt + C - 1) / C + 0.5);
+    if (!h.g || cost < best) best = cost, h.g = g, h.C = C, h.passes = passes;
+  }
+  return h;
+}
+
+static size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Places of the launch's arrays in a workspace; `base` null: its size.
+static size_t head_layout(const HeadPlan &h, int64_t T, int64_t K, int k, uint8_t *base, HeadParams &p, int8_t *&q,
+                          float *&sx) {
+  size_t n = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t *at = base + n;
+    n += up(bytes);
+    return at;
+  };
+  const size_t cells = (size_t)h.parts() * (size_t)h.Tp;
+  sx = (float *)take(sizeof(float) * (size_t)T);
+  q = (int8_t *)take((size_t)T * (size_t)((K + 15) / 16 * 16));
+  p.part_r = (float *)take(sizeof(float) * cells);
+  p.part_s = (float *)take(sizeof(float) * cells);
+  p.part_t = (float *)take(sizeof(float) * cells);
+  if (k > 0) {
+    p.part_best = (key_t *)take(sizeof(key_t) * cells);
+    p.part_n = (int32_t *)take(sizeof(int32_t) * cells);
+    p.part_v = (float *)take(sizeof(float) * cells * (size_t)k);
+    p.part_i = (int32_t *)take(sizeof(int32_t) * cells * (size_t)k);
+    const size_t work = (size_t)h.blocks() * H_CAP * G_EPI_THREADS;
+    p.list_v = (float *)take(sizeof(float) * work);
+    p.list_i = (int32_t *)take(sizeof(int32_t) * work);
+  }
+  return n;
+}
+
+// All tokens, in launches of equal size of at most H_TOKENS.
+static int64_t head_chunk(int64_t T) {
+  const int64_t n = (T + H_TOKENS - 1) / H_TOKENS, c = (T + n - 1) / n;
+  return n == 1 ? T : (c + 255) / 256 * 256;
+}
+
+size_t head_workspace_bytes(const har_cuda_i8_weights *w, int64_t T, int k) {
+  HeadParams p = {};
+  int8_t *q;
+  float *sx;
+  const int64_t c = head_chunk(T), rest = T % c;
+  const size_t most = head_layout(head_plan(c, w->N, w->sms), c, w->K, k, nullptr, p, q, sx);
+  // the last launch is shorter, but its plan may have more parts
+  return rest ? std::max(most, head_layout(head_plan(rest, w->N, w->sms), rest, w->K, k, nullptr, p, q, sx)) : most;
+}
+
+int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
+                       int64_t T, const LogprobOut &out, uint8_t *workspace) {
+  const int k = out.top_ids || out.top_logprobs ? out.k : 0;
+  const int64_t chunk = head_chunk(T), ldq = (w->K + 15) / 16 * 16;
+  for (int64_t t0 = 0; t0 < T; t0 += chunk) {
+    const int64_t n = std::min(chunk, T - t0);
+    const HeadPlan h = head_plan(n, w->N, w->sms);
+    HeadJoin j = {};
+    HeadParams &p = j.p;
+    int8_t *q;
+    float *sx;
+    head_layout(h, n, w->K, k, workspace, p, q, sx);
+    const uint8_t *xs = (const uint8_t *)x + (size_t)(t0 * ldx) * dtype_bytes(x_dtype);
+    int32_t st = launch_i8_quantize(ctx, xs, x_dtype, n, w->K, ldx, q, ldq, sx);
+    if (st != HAR_CUDA_OK) return st;
+    p.sh.K = w->K;
+    p.sh.bn = G_A * h.cg;
+    p.sh.stages = h.cg == 2 ? ring_stages<2>(p.sh.bn) : ring_stages<1>(p.sh.bn);
+    p.T = n, p.V = w->N, p.Tp = h.Tp, p.sx = sx, p.sw = w->scale;
+    p.tt = h.tt, p.vt = h.vt, p.g = h.g, p.C = h.C, p.k = k, p.status = ctx->d_status;
+    TmaDesc map_x;
+    st = encode_tmap_2d(ctx, &map_x, q, 1, (uint64_t)n, (uint64_t)w->K, (uint64_t)ldq, G_A, G_KS, true);
+    if (st != HAR_CUDA_OK) return st;
+    const size_t smem = G_STAGE_BYTES + 1024;
+    prof_begin(ctx);
+    cudaError_t e = h.cg == 2 ? launch_clusters(i8_head_kernel<2>, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 2, map_x, w->map, p)
+                              : launch_clusters(i8_head_kernel<1>, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 1, map_x, w->map, p);
+    st = check_launch(ctx, "i8_head_kernel");
+    if (e != cudaSuccess)
+      return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_kernel: ") + cudaGetErrorString(e));
+    if (st != HAR_CUDA_OK) return st;
+    j.out = out;
+    if (j.out.tokens) j.out.tokens += t0 * out.G;
+    if (j.out.logprobs) j.out.logprobs += t0 * out.G;
+    if (j.out.entropy) j.out.entropy += t0;
+    if (j.out.top_ids) j.out.top_ids += t0 * out.k;
+    if (j.out.top_logprobs) j.out.top_logprobs += t0 * out.k;
+    j.x = q, j.w = w->q, j.ldx = ldq, j.ldw = w->ldq, j.K = w->K, j.parts = h.parts();
+    prof_begin(ctx);
+    if (j.parts <= H_JOIN) head_join_kernel<H_JOIN><<<(unsigned)n, H_JOIN, 0, ctx->stream>>>(j);
+    else head_join_kernel<H_JOIN_MOST><<<(unsigned)n, H_JOIN_MOST, 0, ctx->stream>>>(j);
+    st = check_launch(ctx, "head_join_kernel");
+    if (st != HAR_CUDA_OK) return st;
+  }
+  return HAR_CUDA_OK;
+}
+
+}  // namespace har

@@ -1,57 +1,15 @@
 // k_logprobs.cu — log probabilities of given tokens, entropy and the largest
-// alternatives of each row of logits, in one pass over the row:
-//   s = sum exp(x - r),  t = sum exp(x - r) (x - r)  for a reference r near the
-// row's maximum, so log p = (x - r) - log s and H = log s - t / s whatever r is.
+// alternatives of each row of logits, in one pass over the row.
 #include <algorithm>
 #include <cooperative_groups.h>
 
-#include "topk_warp.cuh"
+#include "logprob_row.cuh"
 
 namespace har {
 
 namespace cg = cooperative_groups;
 
 constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_SEG = 32, LP_MAX_CLUSTER = 16;
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-// Sums about a reference: r starts at -inf (nothing seen but -inf and NaN).
-struct Stat {
-  float r, s, t;
-};
-// Moves the sums to reference r (>= a.r).  From -inf the sums are 0, or NaN.
-__device__ __forceinline__ void stat_move(Stat &a, float r) {
-  if (a.r == r) return;
-  const float d = a.r - r, f = ex2(d * LOG2E);
-  const float shift = a.r == -INFINITY ? 0.0f : f == 0.0f ? 0.0f : d;
-  a.t = f * fmaf(shift, a.s, a.t);
-  a.s = f * a.s;
-  a.r = r;
-}
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
-  const float r = fmaxf(a.r, b.r);
-  stat_move(a, r);
-  stat_move(b, r);
-  return {r, a.s + b.s, a.t + b.t};
-}
-__device__ __forceinline__ Stat warp_stat(Stat a) {
-  float r = a.r;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
-  stat_move(a, r);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
-    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
-  }
-  return a;
-}
-
 // One 16-byte piece of a row.
 template <typename T>
 struct Piece {
@@ -94,32 +52,6 @@ __device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
   const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&raw);
   const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
   return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
-}
-
-// Adds a trip's pieces, whose largest element is `top`, to the sums.  The
-// reference follows the maximum only once it is left behind by more than 6
-// (e^6 = 403 a term at most): a move costs an exponential, and close behind
-// the maximum it would run at almost every trip.
-template <typename T>
-__device__ __forceinline__ void stat_add(Stat &a, const Piece<T> (&p)[LP_U], float top) {
-  if (top > a.r + 6.0f) stat_move(a, top);
-  const float r = a.r == -INFINITY ? 0.0f : a.r;
-  const float2 nr = make_float2(-r, -r), l2e = make_float2(LOG2E, LOG2E);
-  float2 s = make_float2(a.s, 0.0f), t = make_float2(a.t, 0.0f);
-#pragma unroll
-  for (int u = 0; u < LP_U; ++u)
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; i += 2) {
-      float2 d = __fadd2_rn(make_float2(p[u].at(i), p[u].at(i + 1)), nr);
-      d.x = max_nan(d.x, -1e4f);  // -inf (0 times it would be NaN) and all that underflows
-      d.y = max_nan(d.y, -1e4f);
-      const float2 g = __fmul2_rn(d, l2e);
-      const float2 e = make_float2(ex2(g.x), ex2(g.y));
-      s = __fadd2_rn(s, e);
-      t = __ffma2_rn(e, d, t);
-    }
-  a.s = s.x + s.y;
-  a.t = t.x + t.y;
 }
 
 // A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
@@ -192,7 +124,7 @@ __global__ void __launch_bounds__(LP_T, 4)
       for (int u = 1; u < LP_U; ++u) top = fmaxf(top, p[u].top());
       group_top[s][tid] = top;
       most = fmaxf(most, top);
-      stat_add(st, p, top);
+      stat_add<LP_U * N>(st, top, [&](int i) { return p[i / N].at(i % N); });
     }
     if (!want_top) continue;
     // the bound: -inf itself never enters (an empty place is filled at the end)
@@ -246,11 +178,8 @@ __global__ void __launch_bounds__(LP_T, 4)
     st = part_stats[0];
   }
 
-  // an empty row has no reference; a NaN or +inf makes s NaN
-  const bool empty = st.r == -INFINITY && st.s == 0.0f;
-  const float logz = empty ? 0.0f : logf(st.s);
-  auto logp = [&](float v) { return empty ? -INFINITY : (v - st.r) - logz; };
-  if (tid == 0 && out.entropy) out.entropy[row] = empty ? 0.0f : logz - st.t / st.s;
+  const RowEnd row_end(st);
+  if (tid == 0 && out.entropy) out.entropy[row] = row_end.entropy;
   if (out.logprobs)
     for (int g = tid; g < out.G; g += LP_T) {
       if (g >= LP_T) {
@@ -259,7 +188,7 @@ __global__ void __launch_bounds__(LP_T, 4)
       }
       float r = 0.0f;
       if (tok >= 0 && tok < V) {
-        r = logp(given);
+        r = row_end.logp(given);
       } else if (tok != -1) {
         r = __int_as_float(0x7fffffff);
         atomicOr(out.status, DEV_ERR_BOUNDS);
@@ -268,7 +197,7 @@ __global__ void __launch_bounds__(LP_T, 4)
     }
   if (want_top && warp == 0) {
     int id = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
-    float lp = best ? logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
+    float lp = best ? row_end.logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
     // places left: the first masked elements, then the first NaN
     int have = __popc(__ballot_sync(0xffffffffu, best != 0));
     for (int pass = 0; pass < 2 && have < out.k; ++pass)

@@ -162,7 +162,7 @@ int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32
   }
   w->q = (const int8_t *)d;
   w->scale = (const float *)((uint8_t *)d + qb);
-  w->N = N, w->K = K, w->ldq = ldq, w->device = ctx->device, w->owned = true;
+  w->N = N, w->K = K, w->ldq = ldq, w->device = ctx->device, w->sms = ctx->num_sms, w->owned = true;
   return finish_i8_weights(ctx, w, out);
 }
 
@@ -178,7 +178,7 @@ int32_t har_cuda_i8_weights_wrap(har_cuda_ctx *ctx, const int8_t *q_dev, int64_t
   if (!w) return set_error(ctx, HAR_CUDA_ERR_OOM, "i8_weights_wrap: out of host memory");
   w->q = q_dev;
   w->scale = scale_dev;
-  w->N = N, w->K = K, w->ldq = N == 1 ? (int64_t)round16((size_t)K) : ldq, w->device = ctx->device;
+  w->N = N, w->K = K, w->ldq = N == 1 ? (int64_t)round16((size_t)K) : ldq, w->device = ctx->device, w->sms = ctx->num_sms;
   return finish_i8_weights(ctx, w, out);
 }
 
@@ -276,13 +276,9 @@ int32_t har_cuda_token_logprobs(har_cuda_ctx *ctx, const void *logits_dev, int32
   return launch_token_logprobs(ctx, logits_dev, dtype, T, V, T == 1 ? V : ldl, o);
 }
 
-// Rows whose logits are held at a time.
-static int64_t head_rows(int64_t T) { return T < 128 ? T : 128; }
-
 int64_t har_cuda_i8_head_workspace(const har_cuda_i8_weights *w, int64_t T, int32_t G, int32_t k) {
   if (!w || T < 0 || T > I8_MAX_ROWS || G < 0 || k < 0 || k > I8_MAX_TOP) return -1;
-  if (T == 0) return 0;
-  return (int64_t)(quantized_bytes(w, T) + (size_t)head_rows(T) * (size_t)w->N * sizeof(float));
+  return T == 0 ? 0 : (int64_t)head_workspace_bytes(w, T, k);
 }
 
 int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *w,
@@ -294,7 +290,7 @@ int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *
   if (!ctx) return HAR_CUDA_ERR_ARG;
   HAR_TRY(check_i8_weights(ctx, w, "i8_head_logprobs"));
   HAR_TRY(check_dtype(ctx, x_dtype, "i8_head_logprobs"));
-  LogprobOut o = {tokens_dev, G, k, logprobs_dev, entropy_dev, top_logprobs_dev, top_ids_dev, ctx->d_status};
+  const LogprobOut o = {tokens_dev, G, k, logprobs_dev, entropy_dev, top_logprobs_dev, top_ids_dev, ctx->d_status};
   HAR_TRY(check_logprobs(ctx, T, w->N, o, "i8_head_logprobs"));
   if (T == 0) return HAR_CUDA_OK;
   HAR_TRY(check_rows(ctx, x_dev, dtype_bytes(x_dtype), T, w->K, ldx, false, "i8_head_logprobs: x"));
@@ -302,26 +298,8 @@ int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *
   HAR_TRY(on.status(ctx));
   if (T == 1) ldx = w->K;
   uint8_t *ws;
-  HAR_TRY(take_workspace(ctx, workspace_dev, workspace_bytes, (size_t)har_cuda_i8_head_workspace(w, T, G, k),
-                         "i8_head_logprobs", &ws));
-  float *scale = (float *)ws;
-  int8_t *q = (int8_t *)ws + round16(sizeof(float) * (size_t)T);
-  const int64_t ldq = (int64_t)round16((size_t)w->K);
-  float *logits = (float *)((uint8_t *)q + (size_t)T * (size_t)ldq);
-  HAR_TRY(launch_i8_quantize(ctx, x_dev, x_dtype, T, w->K, ldx, q, ldq, scale));
-  const int64_t step = head_rows(T);
-  for (int64_t t0 = 0; t0 < T; t0 += step) {
-    const int64_t n = T - t0 < step ? T - t0 : step;
-    HAR_TRY(launch_i8_matmul(ctx, w, q + t0 * ldq, ldq, scale + t0, n, logits, HAR_CUDA_DTYPE_F32, w->N));
-    LogprobOut c = o;
-    if (c.tokens) c.tokens += t0 * G;
-    if (c.logprobs) c.logprobs += t0 * G;
-    if (c.entropy) c.entropy += t0;
-    if (c.top_ids) c.top_ids += t0 * k;
-    if (c.top_logprobs) c.top_logprobs += t0 * k;
-    HAR_TRY(launch_token_logprobs(ctx, logits, HAR_CUDA_DTYPE_F32, n, w->N, w->N, c));
-  }
-  return HAR_CUDA_OK;
+  HAR_TRY(take_workspace(ctx, workspace_dev, workspace_bytes, head_workspace_bytes(w, T, k), "i8_head_logprobs", &ws));
+  return launch_i8_head(ctx, w, x_dev, x_dtype, ldx, T, o, ws);
 }
 
 }  // extern "C"

@@ -12,7 +12,7 @@ struct har_cuda_i8_weights {
   const int8_t *q = nullptr;
   const float *scale = nullptr;
   int64_t N = 0, K = 0, ldq = 0;
-  int device = 0;
+  int device = 0, sms = 148;
   bool owned = false;  // q and scale share one allocation, at q
   // TMA map of q for the tensor-core kernels: boxes of 128 rows x 128 bytes
   TmaDesc map;
@@ -128,6 +128,10 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
 bool i8_gemv_takes(int64_t M, int64_t K);
 int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype,
                        int64_t ldx, const float *sx, int64_t M, void *y, int32_t y_dtype, int64_t ldy);
+// The whole head call on a workspace of head_workspace_bytes.
+size_t head_workspace_bytes(const har_cuda_i8_weights *w, int64_t T, int k);
+int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
+                       int64_t T, const LogprobOut &out, uint8_t *workspace);
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
                               int64_t V, int64_t ldl, const LogprobOut &out);
 
