@@ -9,19 +9,27 @@
 
 namespace har {
 
-// A block's tile is 128 tokens (tensor-memory lanes) x 128 CG vocabulary rows
-// (columns): a thread of the epilogue owns one token and half the columns, and
-// keeps the token's sums and list to itself.
-constexpr int H_CAP = 96;          // entries of a thread's list: 64, and 32 of the columns in hand
-constexpr int H_FULL = H_CAP - 32;
+// A pair of blocks works on tiles of 256 tokens (tensor-memory lanes) x 256
+// vocabulary rows (columns): a thread of the epilogue owns one token and half
+// the columns, and keeps the token's sums and list to itself.
+constexpr int H_TILE = 2 * G_A, H_COLS = 128;
+constexpr int H_ROW = 8 * G_EPI_THREADS;  // bytes between two entries of a thread's list
+constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
+// Ring slots and entries of a thread's list, which share a block's memory: a
+// list of 40 leaves four slots, and up to 32 entries one sort cuts it.  Above 22
+// alternatives that leaves too few new entries between two cuts (20 of 2,048 x
+// 131,072 x 2,048 took 586 us with 40 entries and 620 with 60, 32 took 4,100
+// and 740): a list of 60 beside three slots.
+constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
-constexpr int64_t H_TOKENS = 4096; // tokens of one launch
+constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
+constexpr int64_t H_WALK = 128;     // up to here the logits go through memory
 
 struct HeadPlan {
-  int cg, tt, vt, g, C, passes;    // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
-  int64_t Tp;                      // tokens rounded up to tiles
+  int tt, vt, g, C, passes;         // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
+  int64_t Tp;                       // tokens rounded up to tiles
   int parts() const { return 2 * C; }
-  int blocks() const { return g * C * cg; }
+  int blocks() const { return 2 * g * C; }
 };
 
 struct HeadParams {
@@ -29,8 +37,7 @@ struct HeadParams {
   int64_t T, V, Tp;
   const float *sx, *sw;
   int tt, vt, g, C, k;
-  float *list_v;                   // [block][H_CAP][256]: the threads' working lists
-  int32_t *list_i;
+  int full;                        // entries at which a list is cut back: 8 below its room
   // part 2 c + h (stream c, half h of a tile's columns) of token t at [part][t]
   float *part_r, *part_s, *part_t;
   key_t *part_best;                // its largest key, 0: no entry
@@ -40,15 +47,14 @@ struct HeadParams {
   int *status;
 };
 
-// Block (or pair) b works on token tile pass * g + b / C and vocabulary tiles
-// b % C, b % C + C, ...: the g pairs of a stream read the same weights at about
-// the same time, so they come from memory once.
-template <int CG>
+// Pair b works on token tile pass * g + b / C and vocabulary tiles b % C,
+// b % C + C, ...: the g pairs of a stream read the same weights at about the
+// same time, so they come from memory once.
 struct HeadTiles {
   const HeadParams &p;
   int slot, c, pass, v;
   __device__ __forceinline__ explicit HeadTiles(const HeadParams &p_) : p(p_), pass(0) {
-    const int b = blockIdx.x / CG;
+    const int b = blockIdx.x / 2;
     slot = b / p.C;
     c = v = b - slot * p.C;
   }
@@ -59,8 +65,8 @@ struct HeadTiles {
     }
     const int t = pass * p.g + slot;
     if (t >= p.tt) return false;
-    a_row = t * (CG * G_A);
-    b_row = v * (CG * G_A);
+    a_row = t * H_TILE;
+    b_row = v * H_TILE;
     v += p.C;
     return true;
   }
@@ -106,105 +112,119 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
   return r;
 }
 
-struct ListState {
-  int n;
+// A thread's list in shared memory: entries (value, id), H_ROW bytes apart,
+// from `at`; `end` is behind the last, values above `bar` may enter.
+struct List {
+  uint32_t at, end;
   float bar;
+  __device__ __forceinline__ int n() const { return (int)(end - at) / H_ROW; }
 };
-// Cuts a thread's list back to its k largest entries: the k-th value from a
-// sort of the values alone, then one sweep that keeps what is above it and, of
-// its equals, the first (entries stand in the order of their ids).  The whole
-// warp; a thread with fewer than k entries keeps them and its bar.
-__device__ __noinline__ ListState list_cut(float *v, int32_t *id, ListState s, int k) {
-  float top[32], more[32];
-  const int most = __reduce_max_sync(0xffffffffu, s.n);
+__device__ __forceinline__ float list_value(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ int32_t list_id(uint32_t at) {
+  int32_t v;
+  asm volatile("ld.shared.s32 %0, [%1+4];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+// Appends (v, id) if v is above the bar: four instructions and no branch.
+__device__ __forceinline__ void list_push(List &l, float v, int32_t id) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.gt.f32 p, %1, %2;\n\t"
+      "@p st.shared.v2.b32 [%0], {%3, %4};\n\t"
+      "@p add.u32 %0, %0, %5;\n\t}"
+      : "+r"(l.end)
+      : "f"(v), "f"(l.bar), "r"(__float_as_uint(v)), "r"(id), "n"(H_ROW)
+      : "memory");
+}
+// Cuts a list back to its k largest entries: the k-th value from a sort of the
+// values alone, then one sweep that keeps what is above it and, of its equals,
+// the first (entries stand in the order of their ids).  The whole warp; a
+// thread with fewer than k entries keeps them and its bar.
+__device__ __noinline__ List list_cut(List s, int k) {
+  float top[32];
+  const int n = s.n();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top[i] = i < s.n ? v[i * G_EPI_THREADS] : -INFINITY;
+  for (int i = 0; i < 32; ++i) top[i] = i < n ? list_value(s.at + i * H_ROW) : -INFINITY;
   sort32_desc(top);
-  for (int b = 32; b < most; b += 32) {
+  if (__any_sync(0xffffffffu, n > 32)) {
+    float more[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) more[i] = b + i < s.n ? v[(b + i) * G_EPI_THREADS] : -INFINITY;
+    for (int i = 0; i < 32; ++i) more[i] = 32 + i < n ? list_value(s.at + (32 + i) * H_ROW) : -INFINITY;
     sort32_desc(more);
     merge32_desc(top, more);
   }
-  if (s.n < k) return s;
+  if (n < k) return s;
   const float bar = pick32(top, k - 1);
   int equals = k;
 #pragma unroll
   for (int i = 0; i < 32; ++i) equals -= i < k && top[i] > bar;
-  int n = 0;
-  for (int e0 = 0; e0 < s.n; e0 += 8) {
-    float x[8];
-    int32_t y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = e0 + i < s.n ? v[(e0 + i) * G_EPI_THREADS] : -INFINITY;
-      y[i] = e0 + i < s.n ? id[(e0 + i) * G_EPI_THREADS] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool keep = e0 + i < s.n && (x[i] > bar || (x[i] == bar && equals-- > 0));
-      if (keep) {
-        v[n * G_EPI_THREADS] = x[i];
-        id[n * G_EPI_THREADS] = y[i];
-        ++n;
-      }
+  uint32_t end = s.at;
+  for (uint32_t e = s.at; e < s.end; e += H_ROW) {
+    const float x = list_value(e);
+    const int32_t id = list_id(e);
+    if (x > bar || (x == bar && equals-- > 0)) {
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(end), "r"(__float_as_uint(x)), "r"(id) : "memory");
+      end += H_ROW;
     }
   }
-  return {n, bar};
+  return {s.at, end, bar};
 }
 
-template <int CG>
 __global__ void __launch_bounds__(G_THREADS, 1)
     i8_head_kernel(const __grid_constant__ TmaDesc map_x, const __grid_constant__ TmaDesc map_w, const HeadParams p) {
-  constexpr int COLS = 64 * CG;  // a thread's columns of a tile
   extern __shared__ uint8_t g_raw[];
   __shared__ Ring ring;
   __shared__ int go[2][2];
-  __shared__ __align__(16) float scales[2][2][COLS];
+  __shared__ __align__(16) float scales[2][2][H_COLS];
   uint8_t *sm = g_raw + ((1024u - (tc::smem_u32(g_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? tc::cluster_rank() : 0u;
-  ring_open<CG>(ring, p.sh, &map_x, &map_w);
+  const uint32_t rank = tc::cluster_rank();
+  ring_open<2>(ring, p.sh, &map_x, &map_w);
 
   if (warp == G_WARP_A) {
-    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, false, &map_x, HeadTiles<CG>(p), rank);
+    if (lane == 0) ring_produce<2>(ring, p.sh, sm, false, &map_x, HeadTiles(p), rank);
   } else if (warp == G_WARP_B) {
-    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, true, &map_w, HeadTiles<CG>(p), rank);
+    if (lane == 0) ring_produce<2>(ring, p.sh, sm, true, &map_w, HeadTiles(p), rank);
   } else if (warp == G_WARP_MMA) {
-    if (rank == 0) ring_issue<CG>(ring, p.sh, sm, HeadTiles<CG>(p));
+    if (rank == 0) ring_issue<2>(ring, p.sh, sm, HeadTiles(p));
   } else {
     volatile int *abort_s = &ring.abort_flag;
     const int quad = warp & 3, h = (warp - G_WARP_EPI) >> 2;
-    const int row = 32 * quad + lane, me = h * 128 + row;
-    const uint32_t col0 = ring.tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(h * COLS);
-    float *lv = p.list_v + (int64_t)blockIdx.x * (H_CAP * G_EPI_THREADS) + me;
-    int32_t *li = p.list_i + (int64_t)blockIdx.x * (H_CAP * G_EPI_THREADS) + me;
-    HeadTiles<CG> tiles(p);
+    const int row = 32 * quad + lane;
+    const uint32_t col0 = ring.tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(h * H_COLS);
+    HeadTiles tiles(p);
     Stat st = {-INFINITY, 0.0f, 0.0f};
-    ListState ls = {0, INFINITY};
+    List ls;
+    ls.at = ls.end = tc::smem_u32(sm + p.sh.stages * H_SLOT) + 8u * (uint32_t)(128 * h + row);
+    ls.bar = INFINITY;
     int64_t token = -1;
     float sx = 0.0f;
     int cur = -1;
 
     // the token tile's part is done
     auto flush = [&]() {
-      if (p.k > 0) ls = list_cut(lv, li, ls, p.k);
+      if (p.k > 0) ls = list_cut(ls, p.k);
       if (token >= p.T) return;
-      const int64_t at = (int64_t)(2 * tiles.c + h) * p.Tp + token;
+      const int64_t part = 2 * tiles.c + h, at = part * p.Tp + token;
       p.part_r[at] = st.r;
       p.part_s[at] = st.s;
       p.part_t[at] = st.t;
       if (p.k == 0) return;
       key_t best = 0;
-      for (int e = 0; e < ls.n; ++e) {
-        const float x = lv[e * G_EPI_THREADS];
-        const int32_t id = li[e * G_EPI_THREADS];
-        const int64_t to = ((int64_t)(2 * tiles.c + h) * p.k + e) * p.Tp + token;
+      const int n = ls.n();
+      for (int e = 0; e < n; ++e) {
+        const float x = list_value(ls.at + e * H_ROW);
+        const int32_t id = list_id(ls.at + e * H_ROW);
+        const int64_t to = (part * p.k + e) * p.Tp + token;
         p.part_v[to] = x;
         p.part_i[to] = id;
         best = key_max(best, order_key(x, (uint32_t)id));
       }
-      p.part_n[at] = ls.n;
+      p.part_n[at] = n;
       p.part_best[at] = best;
     };
 
@@ -215,14 +235,17 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       if (a_row != cur) {
         if (cur >= 0) flush();
         cur = a_row;
-        first = true;
+        first = p.k > 0;
         token = (int64_t)a_row + rank * G_A + row;
         sx = token < p.T ? __ldg(p.sx + token) : 0.0f;
         st = {-INFINITY, 0.0f, 0.0f};
-        ls = {0, token < p.T ? -INFINITY : INFINITY};
+        ls.end = ls.at;
+        ls.bar = token < p.T ? -INFINITY : INFINITY;
       }
-      const int64_t v0 = (int64_t)b_row + h * COLS;  // this half's first vocabulary row
-      if (row < COLS) scales[a][h][row] = v0 + row < p.V ? __ldg(p.sw + v0 + row) : 0.0f;
+      const int64_t v0 = (int64_t)b_row + h * H_COLS;  // this half's first vocabulary row
+      scales[a][h][row] = v0 + row < p.V ? __ldg(p.sw + v0 + row) : 0.0f;
+      // one warp waits for the half and says whether to go on, so that all four
+      // leave together when a wait gave up
       if (quad == 0) {
         const bool ok = g_wait_warp(ring.acc_full + a, (n >> 1) & 1u, abort_s, lane, 256);
         if (lane == 0) go[h][a] = ok;
@@ -234,11 +257,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       }
       tc::tc_fence_after();
       const uint32_t col = col0 + a * 256u;
-      const bool ragged = v0 + COLS > p.V;
+      const int width = (int)min((int64_t)H_COLS, p.V - v0);  // columns within V
+      uint32_t v[32];
       // 32 logits from column c on, as i8_linear writes them; -inf past V
       auto logits = [&](int c, float (&l)[32]) {
-        uint32_t v[32];
-        tc::tmem_ld32(col + (uint32_t)c, v);
         tc::tmem_wait_ld32(v);
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -248,57 +270,58 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           l[i + 2] = __fmul_rn(__int2float_rn((int)v[i + 2]), __fmul_rn(sx, s.z));
           l[i + 3] = __fmul_rn(__int2float_rn((int)v[i + 3]), __fmul_rn(sx, s.w));
         }
-        if (ragged) {
+        if (c + 32 > width) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) l[i] = v0 + c + i < p.V ? l[i] : -INFINITY;
+          for (int i = 0; i < 32; ++i) l[i] = c + i < width ? l[i] : -INFINITY;
         }
       };
-      if (first && p.k > 0) {
+      if (first) {
         // the k-th largest of 32 groups' largest logits: k logits are at least
         // as large, so the list starts behind a float below them
         float top[32];
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
+        for (int c = 0; c < H_COLS; c += 32) {
           float l[32];
+          tc::tmem_ld32(col + (uint32_t)c, v);
           logits(c, l);
-          constexpr int W = COLS / 32;  // columns of a group
 #pragma unroll
-          for (int i = 0; i < 32; i += W) {
-            float m = l[i];
-#pragma unroll
-            for (int j = 1; j < W; ++j) m = fmaxf(m, l[i + j]);
-            top[(c + i) / W] = fmaxf(m, -INFINITY);
-          }
+          for (int i = 0; i < 32; i += 4)
+            top[(c + i) / 4] = fmaxf(fmaxf(fmaxf(l[i], l[i + 1]), fmaxf(l[i + 2], l[i + 3])), -INFINITY);
         }
         sort32_desc(top);
         const uint32_t o = order_bits(pick32(top, p.k - 1));
         // two steps down: the one below +0 is -0, its equal
         if (token < p.T) ls.bar = order_value(max(o - 2u, order_bits(-INFINITY)));
       }
-#pragma unroll
-      for (int c = 0; c < COLS; c += 32) {
+      tc::tmem_ld32(col, v);
+#pragma unroll 1
+      for (int c = 0; c < H_COLS; c += 32) {
         float l[32];
         logits(c, l);
-        if (c + 32 == COLS) ring_release<CG>(ring, a, lane);
-        float top = l[0];
+        if (c + 32 < H_COLS) tc::tmem_ld32(col + (uint32_t)(c + 32), v);
+        else ring_release<2>(ring, a, lane);
+        float top[4];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) top = fmaxf(top, l[i]);
-        if (p.k > 0 && __any_sync(0xffffffffu, top > ls.bar)) {
+        for (int q = 0; q < 4; ++q) {
+          top[q] = l[8 * q];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (l[i] > ls.bar) {
-              lv[ls.n * G_EPI_THREADS] = l[i];
-              li[ls.n * G_EPI_THREADS] = (int32_t)(v0 + c + i);
-              ++ls.n;
-            }
-          if (__any_sync(0xffffffffu, ls.n > H_FULL)) ls = list_cut(lv, li, ls, p.k);
+          for (int i = 1; i < 8; ++i) top[q] = fmaxf(top[q], l[8 * q + i]);
         }
-        stat_add<32>(st, top, [&](int i) { return l[i]; });
+        if (p.k > 0) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (__any_sync(0xffffffffu, top[q] > ls.bar)) {
+#pragma unroll
+              for (int i = 8 * q; i < 8 * q + 8; ++i) list_push(ls, l[i], (int32_t)v0 + c + i);
+              if (__any_sync(0xffffffffu, ls.n() > p.full)) ls = list_cut(ls, p.k);
+            }
+        }
+        stat_add<32>(st, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), [&](int i) { return l[i]; });
       }
     }
     if (cur >= 0) flush();
   }
-  ring_close<CG>(ring, p.status);
+  ring_close<2>(ring, p.status);
 }
 
 // ---- joining the parts --------------------------------------------------------------
@@ -427,15 +450,14 @@ __global__ void __launch_bounds__(TH) head_join_kernel(const HeadJoin j) {
 
 // ---- host ---------------------------------------------------------------------------
 
-// Pairs of blocks above 128 tokens.  Token tiles at a time: the number that
-// takes the fewest steps of a tile, more of them (fewer parts) for equal steps.
+// Token tiles at a time: the number that takes the fewest steps of a tile,
+// more of them (fewer parts) for equal steps.
 static HeadPlan head_plan(int64_t T, int64_t V, int sms) {
   HeadPlan h = {};
-  h.cg = T > G_A ? 2 : 1;
-  const int tile = G_A * h.cg, slots = sms / h.cg;
-  h.tt = (int)((T + tile - 1) / tile);
-  h.vt = (int)((V + tile - 1) / tile);
-  h.Tp = (int64_t)h.tt * tile;
+  const int slots = sms / 2;
+  h.tt = (int)((T + H_TILE - 1) / H_TILE);
+  h.vt = (int)((V + H_TILE - 1) / H_TILE);
+  h.Tp = (int64_t)h.tt * H_TILE;
   double best = 0;
   for (int g = std::min(h.tt, slots); g >= 1; --g) {
     const int C = std::min({h.vt, slots / g, H_JOIN_MOST / 2}), passes = (h.tt + g - 1) / g;
@@ -467,9 +489,6 @@ static size_t head_layout(const HeadPlan &h, int64_t T, int64_t K, int k, uint8_
     p.part_n = (int32_t *)take(sizeof(int32_t) * cells);
     p.part_v = (float *)take(sizeof(float) * cells * (size_t)k);
     p.part_i = (int32_t *)take(sizeof(int32_t) * cells * (size_t)k);
-    const size_t work = (size_t)h.blocks() * H_CAP * G_EPI_THREADS;
-    p.list_v = (float *)take(sizeof(float) * work);
-    p.list_i = (int32_t *)take(sizeof(int32_t) * work);
   }
   return n;
 }
@@ -477,21 +496,50 @@ static size_t head_layout(const HeadPlan &h, int64_t T, int64_t K, int k, uint8_
 // All tokens, in launches of equal size of at most H_TOKENS.
 static int64_t head_chunk(int64_t T) {
   const int64_t n = (T + H_TOKENS - 1) / H_TOKENS, c = (T + n - 1) / n;
-  return n == 1 ? T : (c + 255) / 256 * 256;
+  return n == 1 ? T : (c + H_TILE - 1) / H_TILE * H_TILE;
+}
+
+// The logits of a few rows go through memory: scales, q, logits.
+static size_t walk_layout(int64_t T, int64_t V, int64_t K, uint8_t *base, int8_t *&q, float *&sx, float *&logits) {
+  sx = (float *)base;
+  q = (int8_t *)(base + up(sizeof(float) * (size_t)T));
+  const size_t before = up(sizeof(float) * (size_t)T) + up((size_t)T * (size_t)((K + 15) / 16 * 16));
+  logits = (float *)(base + before);
+  return before + sizeof(float) * (size_t)T * (size_t)((V + 3) / 4 * 4);
 }
 
 size_t head_workspace_bytes(const har_cuda_i8_weights *w, int64_t T, int k) {
   HeadParams p = {};
   int8_t *q;
-  float *sx;
+  float *sx, *logits;
+  if (T <= H_WALK) return walk_layout(T, w->N, w->K, nullptr, q, sx, logits);
   const int64_t c = head_chunk(T), rest = T % c;
   const size_t most = head_layout(head_plan(c, w->N, w->sms), c, w->K, k, nullptr, p, q, sx);
   // the last launch is shorter, but its plan may have more parts
   return rest ? std::max(most, head_layout(head_plan(rest, w->N, w->sms), rest, w->K, k, nullptr, p, q, sx)) : most;
 }
 
+// Up to 128 tokens a pair would spend as much of its loads on the token tile
+// as on the weights; the logits stay in L2 instead.
+static int32_t head_walk(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
+                         int64_t T, const LogprobOut &out, uint8_t *workspace) {
+  int8_t *q;
+  float *sx, *logits;
+  walk_layout(T, w->N, w->K, workspace, q, sx, logits);
+  const int64_t ldq = (w->K + 15) / 16 * 16, ldl = (w->N + 3) / 4 * 4;
+  int32_t st;
+  if (i8_gemv_takes(T, w->K)) {
+    st = launch_i8_gemv(ctx, w, x, x_dtype, ldx, nullptr, T, logits, HAR_CUDA_DTYPE_F32, ldl);
+  } else {
+    st = launch_i8_quantize(ctx, x, x_dtype, T, w->K, ldx, q, ldq, sx);
+    if (st == HAR_CUDA_OK) st = launch_i8_matmul(ctx, w, q, ldq, sx, T, logits, HAR_CUDA_DTYPE_F32, ldl);
+  }
+  return st != HAR_CUDA_OK ? st : launch_token_logprobs(ctx, logits, HAR_CUDA_DTYPE_F32, T, w->N, ldl, out);
+}
+
 int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
                        int64_t T, const LogprobOut &out, uint8_t *workspace) {
+  if (T <= H_WALK) return head_walk(ctx, w, x, x_dtype, ldx, T, out, workspace);
   const int k = out.top_ids || out.top_logprobs ? out.k : 0;
   const int64_t chunk = head_chunk(T), ldq = (w->K + 15) / 16 * 16;
   for (int64_t t0 = 0; t0 < T; t0 += chunk) {
@@ -506,17 +554,19 @@ int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     int32_t st = launch_i8_quantize(ctx, xs, x_dtype, n, w->K, ldx, q, ldq, sx);
     if (st != HAR_CUDA_OK) return st;
     p.sh.K = w->K;
-    p.sh.bn = G_A * h.cg;
-    p.sh.stages = h.cg == 2 ? ring_stages<2>(p.sh.bn) : ring_stages<1>(p.sh.bn);
+    p.sh.bn = H_TILE;
+    const int cap = k > H_LONG ? H_CAP_LONG : H_CAP;
+    p.sh.stages = k > H_LONG ? H_SLOTS_LONG : H_SLOTS;
+    // early cuts pay: a list is cut at twice its length, and not before 8 new
+    p.full = std::min(cap - 8, std::max(2 * k, k + 8));
     p.T = n, p.V = w->N, p.Tp = h.Tp, p.sx = sx, p.sw = w->scale;
     p.tt = h.tt, p.vt = h.vt, p.g = h.g, p.C = h.C, p.k = k, p.status = ctx->d_status;
     TmaDesc map_x;
     st = encode_tmap_2d(ctx, &map_x, q, 1, (uint64_t)n, (uint64_t)w->K, (uint64_t)ldq, G_A, G_KS, true);
     if (st != HAR_CUDA_OK) return st;
-    const size_t smem = G_STAGE_BYTES + 1024;
+    const size_t smem = (size_t)p.sh.stages * H_SLOT + (size_t)cap * H_ROW + 1024;
     prof_begin(ctx);
-    cudaError_t e = h.cg == 2 ? launch_clusters(i8_head_kernel<2>, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 2, map_x, w->map, p)
-                              : launch_clusters(i8_head_kernel<1>, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 1, map_x, w->map, p);
+    const cudaError_t e = launch_clusters(i8_head_kernel, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 2, map_x, w->map, p);
     st = check_launch(ctx, "i8_head_kernel");
     if (e != cudaSuccess)
       return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_kernel: ") + cudaGetErrorString(e));

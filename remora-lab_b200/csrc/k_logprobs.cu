@@ -10,6 +10,7 @@ namespace har {
 namespace cg = cooperative_groups;
 
 constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_SEG = 32, LP_MAX_CLUSTER = 16;
+constexpr int LP_QUEUE = 256, LP_CAND = 512;
 // One 16-byte piece of a row.
 template <typename T>
 struct Piece {
@@ -57,17 +58,21 @@ __device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
 // A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
 // part of its pieces, walked in trips of LP_T x LP_U pieces.  The alternatives
 // cost the walk one store: a thread notes the largest element of each trip (a
-// group of LP_U pieces).  After up to LP_SEG trips the k-th largest of the
-// threads' largest elements bounds the k-th largest of all from below, so only
-// groups that reach it (about k of thousands) can hold an alternative; a warp
-// reads its own again, from L2, one element a lane, into its sorted list.
+// group of LP_U pieces).  After up to LP_SEG trips a bound is taken that at
+// least k of the threads' largest elements reach, so only groups that reach it
+// (k or a few more of thousands) can hold an alternative: they are queued, read
+// again from L2, one element a lane, and the elements that reach the bound are
+// sorted.  Where ties are so many that the queue overflows, each warp goes
+// through its own groups in order instead.
 template <typename T>
 __global__ void __launch_bounds__(LP_T, 4)
     token_logprobs_kernel(const T *__restrict__ logits, int64_t V, int64_t ldl, LogprobOut out, int C) {
   constexpr int N = Piece<T>::N;
   __shared__ float group_top[LP_SEG][LP_T];
-  __shared__ uint32_t tops[LP_WARPS][32];
-  __shared__ uint32_t bound_s;
+  __shared__ uint32_t warp_top[LP_WARPS], least_s;
+  __shared__ int queued, found;
+  __shared__ int queue[LP_QUEUE];
+  __shared__ key_t cand[LP_CAND];
   __shared__ key_t lists[LP_MAX_CLUSTER][32];  // the block's lists, then the cluster's
   __shared__ key_t part_list[LP_WARPS][32];
   __shared__ Stat stats[LP_WARPS], part_stats[LP_MAX_CLUSTER];
@@ -106,8 +111,8 @@ __global__ void __launch_bounds__(LP_T, 4)
     }
   };
   Stat st = {-INFINITY, 0.0f, 0.0f};
-  key_t list = 0;
-  float bar = -INFINITY;  // the k-th entry's value, once there are k
+  key_t best = 0;  // warp 0: the row's largest so far
+  if (tid == 0) queued = found = 0, least_s = order_bits(-INFINITY) + 1u;  // -inf never enters: see the end
   Piece<T> next[LP_U];
   if (j0 < j1) load_trip(next, j0);
   for (int64_t seg = j0; seg < j1; seg += (int64_t)LP_SEG * LP_T * LP_U) {
@@ -127,14 +132,59 @@ __global__ void __launch_bounds__(LP_T, 4)
       stat_add<LP_U * N>(st, top, [&](int i) { return p[i / N].at(i % N); });
     }
     if (!want_top) continue;
-    // the bound: -inf itself never enters (an empty place is filled at the end)
-    tops[warp][lane] = warp_sort_desc(order_bits(most), lane);
+    // each warp's ceil(k / 8)-th largest thread: together at least k elements
+    // reach the smallest of the eight
+    const uint32_t sorted = warp_sort_desc(order_bits(most), lane);
+    if (lane == (out.k + LP_WARPS - 1) / LP_WARPS - 1) warp_top[warp] = sorted;
     __syncthreads();
-    const uint32_t merged = block_merge_lists(tops, LP_WARPS, warp, lane);
-    if (warp == 0 && lane == out.k - 1) bound_s = max(merged, order_bits(-INFINITY) + 1u);
+    uint32_t bound = warp_top[0];
+#pragma unroll
+    for (int w = 1; w < LP_WARPS; ++w) bound = min(bound, warp_top[w]);
+    bound = max(bound, least_s);
+    if (order_bits(most) >= bound) {
+#pragma unroll 8
+      for (int s = 0; s < trips; ++s)
+        if (order_bits(group_top[s][tid]) >= bound) {
+          const int at = atomicAdd(&queued, 1);
+          if (at < LP_QUEUE) queue[at] = s * LP_T + tid;
+        }
+    }
     __syncthreads();
-    const uint32_t bound = bound_s;
-    if (__any_sync(0xffffffffu, order_bits(most) >= bound)) {
+    const int nq = queued;
+    // element `lane` of a group, -inf outside the row
+    auto element = [&](int g, int64_t &e) {
+      const int64_t j = seg + (int64_t)(g / LP_T) * (LP_T * LP_U) + g % LP_T + (lane / N) * LP_T;
+      e = j * N - off + lane % N;
+      return lane < LP_U * N && j < j1 && e >= 0 && e < V ? to_f32(x[e]) : -INFINITY;
+    };
+    if (nq <= LP_QUEUE) {
+      for (int i = warp; i < nq; i += 4 * LP_WARPS) {
+        int64_t e[4];
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          v[u] = -INFINITY;
+          if (i + u * LP_WARPS < nq) v[u] = element(queue[i + u * LP_WARPS], e[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (order_bits(v[u]) >= bound) {
+            const int at = atomicAdd(&found, 1);
+            if (at < LP_CAND) cand[at] = order_key(v[u], (uint32_t)e[u]);
+          }
+      }
+    }
+    __syncthreads();
+    const int n = found;
+    key_t list = 0;
+    if (nq <= LP_QUEUE && n <= LP_CAND) {
+      // up to 64: one warp; more: all
+      for (int i = 32 * warp; i < n; i += n <= 64 ? 32 : LP_T) {
+        if (n <= 64 && warp > 0) break;
+        list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? cand[i + lane] : (key_t)0, lane), lane);
+      }
+    } else {
+      float bar = -INFINITY;  // the k-th entry's value, once there are k
       for (int s = 0; s < trips; ++s) {
         const float top = group_top[s][tid];
         // trips come in ascending order: a value equal to the k-th entry of
@@ -142,10 +192,8 @@ __global__ void __launch_bounds__(LP_T, 4)
         uint32_t groups = __ballot_sync(0xffffffffu, order_bits(top) >= bound && top > bar);
         if (!groups) continue;
         for (; groups; groups &= groups - 1) {
-          const int64_t j = seg + (int64_t)s * (LP_T * LP_U) + 32 * warp + (__ffs(groups) - 1) + (lane / N) * LP_T;
-          const int64_t e = j * N - off + lane % N;
-          const bool in = lane < LP_U * N && j < j1 && e >= 0 && e < V;
-          const float v = in ? to_f32(x[e]) : -INFINITY;
+          int64_t e = 0;
+          const float v = element(s * LP_T + 32 * warp + __ffs(groups) - 1, e);
           const key_t key = order_key(v, (uint32_t)e);
           const key_t last = __shfl_sync(0xffffffffu, list, out.k - 1);
           list = warp_take(list, key, __ballot_sync(0xffffffffu, v > -INFINITY && key > last), lane);
@@ -154,12 +202,25 @@ __global__ void __launch_bounds__(LP_T, 4)
         if (last) bar = order_value((uint32_t)(last >> 32));
       }
     }
+    if (nq > LP_QUEUE || n > 64) {
+      part_list[warp][lane] = list;
+      __syncthreads();
+      list = block_merge_lists(part_list, LP_WARPS, warp, lane);
+    }
+    if (warp == 0) {
+      best = seg == j0 ? list : warp_merge_desc(best, list, lane);
+      // what comes later and only equals the k-th entry loses to it
+      const key_t last = __shfl_sync(0xffffffffu, best, out.k - 1);
+      if (lane == 0) {
+        if (last) least_s = max(least_s, (uint32_t)(last >> 32) + 1u);
+        queued = found = 0;
+      }
+    }
+    __syncthreads();
   }
   st = warp_stat(st);
-  if (want_top) part_list[warp][lane] = list;
   if (lane == 0) stats[warp] = st;
   __syncthreads();
-  key_t best = want_top ? block_merge_lists(part_list, LP_WARPS, warp, lane) : 0;
   if (warp == 0) st = warp_stat(lane < LP_WARPS ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
   if (C > 1) {
     cg::cluster_group cl = cg::this_cluster();
@@ -215,15 +276,16 @@ __global__ void __launch_bounds__(LP_T, 4)
   }
 }
 
-// Blocks a row: 1 to 16, a power of two.  592 blocks (4 an SM) run at a time;
-// a block costs its share of the row and about 4,096 elements' time to start
-// and to join.
-static int pick_cluster(int64_t T, int64_t V, int sms) {
+// Blocks a row: 1 to 16, a power of two.  4 blocks an SM run at a time; one
+// takes about 5 us to start, to find its alternatives and to join, and reads
+// 16 KB/us alone or beside another, 11 beside three.
+static int pick_cluster(int64_t T, int64_t bytes, int sms) {
   int best = 1;
   double least = 0;
   for (int c = 1; c <= LP_MAX_CLUSTER; c *= 2) {
-    const int64_t waves = (T * c + 4 * sms - 1) / (4 * sms);
-    const double cost = (double)waves * ((double)V / c + 4096.0);
+    const int64_t blocks = T * c, full = blocks / (4 * sms), rest = blocks % (4 * sms);
+    const double kb = (double)bytes / c / 1000.0;
+    const double cost = full * (5.0 + kb / 11.0) + (rest == 0 ? 0.0 : 5.0 + kb / (rest <= 2 * sms ? 16.0 : 11.0));
     if (c == 1 || cost < least) best = c, least = cost;
   }
   return best;
@@ -231,7 +293,7 @@ static int pick_cluster(int64_t T, int64_t V, int sms) {
 
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
                               int64_t V, int64_t ldl, const LogprobOut &out) {
-  const int C = pick_cluster(T, V, ctx->num_sms);
+  const int C = pick_cluster(T, V * (int64_t)dtype_bytes(dtype), ctx->num_sms);
   cudaError_t e = cudaSuccess;
   // a grid holds 2^31 - 1 blocks
   const int64_t most = ((int64_t)1 << 30) / C;
