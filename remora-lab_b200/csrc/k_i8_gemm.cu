@@ -49,25 +49,32 @@ struct GemmTiles {
   }
 };
 
-// One token's channels from shared memory to unaligned memory, a warp: whole
-// 4-byte words, a 2-byte type's odd first and last element apart.
+// Tokens quad, quad + 4, ... of a slab, from shared memory to rows of any
+// alignment, by one warp: whole 4-byte words, a 2-byte type's odd first and
+// last element apart; four rows on their way at a time.
 template <typename T>
-__device__ __forceinline__ void put_row(T *y, const T *row, int n, int lane) {
-  if (sizeof(T) == 4) {
+__device__ __forceinline__ void put_rows(T *y, int64_t ldy, const T *slab, int tokens, int chans, int quad, int lane) {
+  if (chans <= 0) return;
+#pragma unroll 4
+  for (int t = quad; t < tokens; t += 4) {
+    T *to = y + t * ldy;
+    const T *row = slab + t * G_A;
+    if (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < G_A; i += 32)
-      if (i + lane < n) y[i + lane] = row[i + lane];
-  } else {
-    const int odd = (int)((uintptr_t)y >> 1) & 1;
-    if (odd && n > 0 && lane == 0) y[0] = row[0];
+      for (int i = 0; i < G_A; i += 32)
+        if (i + lane < chans) to[i + lane] = row[i + lane];
+    } else {
+      const int odd = (int)((uintptr_t)to >> 1) & 1;
+      if (odd && lane == 0) to[0] = row[0];
 #pragma unroll
-    for (int i = 0; i < G_A; i += 64) {
-      const int e = odd + i + 2 * lane;
-      if (e + 1 < n) {
-        const T two[2] = {row[e], row[e + 1]};
-        *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(two);
-      } else if (e < n) {
-        y[e] = row[e];
+      for (int i = 0; i < G_A; i += 64) {
+        const int e = odd + i + 2 * lane;
+        if (e + 1 < chans) {
+          const T two[2] = {row[e], row[e + 1]};
+          *reinterpret_cast<uint32_t *>(to + e) = *reinterpret_cast<const uint32_t *>(two);
+        } else if (e < chans) {
+          to[e] = row[e];
+        }
       }
     }
   }
@@ -113,7 +120,7 @@ __device__ __forceinline__ void put_slabs(const GemmParams &p, const void *map_y
     } else {
       T *y = (T *)p.y + (m + i * TOK) * p.ldy + chan0;
       const int chans = (int)min((int64_t)G_A, p.N - chan0);
-      for (int t = quad; t < min(TOK, n - i * TOK); t += 4) put_row(y + t * p.ldy, slab + t * G_A, chans, lane);
+      put_rows(y, p.ldy, slab, min(TOK, n - i * TOK), chans, quad, lane);
     }
   }
 }

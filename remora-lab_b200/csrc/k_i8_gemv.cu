@@ -115,7 +115,13 @@ __global__ void __launch_bounds__(V_T, 2) i8_gemv_kernel(const GemvParams p) {
     for (int k = 4 * t; k < pieces * 16; k += WPR * 128) {
       float v[4];
       load4(p.x, p.x_dtype, x0 + k, live ? (int)p.K - k : 0, p.wide, v);
-      q[k >> 2] = rs.round4(v);
+      if (rs.odd()) {
+        uint32_t w = 0;
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)(uint8_t)rs.round_odd(v[i]) << (8 * i);
+        q[k >> 2] = w;
+      } else {
+        q[k >> 2] = rs.round4(v);
+      }
     }
   }
   __syncthreads();

@@ -45,7 +45,8 @@ def quantized(ctx, x):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("M,K,pad", [(1, 1, 0), (3, 7, 2), (2, 8, 0), (9, 64, 8), (5, 1000, 0), (4, 1024, 0),
-                                     (7, 1025, 0), (3, 2048, 3), (2, 4096, 0), (3, 4104, 8), (2, 16384, 0),
+                                     (7, 1025, 0), (3, 2048, 3), (5, 2049, 0), (2, 4096, 0), (3, 4104, 8), (2, 8192, 0),
+                                     (2, 8200, 0), (2, 16384, 0),
                                      (2, 16397, 0), (1, 40001, 0), (700, 130, 1)])
 def test_quantize_rows(ctx, dtype, M, K, pad):
     x = rows(K * 7 + M, M, K, dtype, pad)
@@ -72,6 +73,26 @@ def test_quantize_halves_zeros_and_extremes(ctx):
     assert torch.equal(s.cpu().nan_to_num(7.0), rs.nan_to_num(7.0))
     assert torch.equal(q.cpu().long(), rq)
     assert s[1] == 0 and not q[1].any() and not q[5].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_quantize_next_to_halves(ctx, dtype):
+    """Every quotient beside a half, for many divisors: x = (n + 1/2) s and its
+    neighbours; the row's largest value fixes s."""
+    g = torch.Generator().manual_seed(3)
+    rows_ = 400
+    top = (torch.rand(rows_, generator=g) + 0.5) * torch.exp2(torch.randint(-12, 12, (rows_,), generator=g).float())
+    top = top.to(DT[dtype]).float()
+    s = top / 127
+    h = torch.arange(-127, 127).float() + 0.5
+    mid = (h.unsqueeze(0) * s.unsqueeze(1)).to(DT[dtype])
+    up = torch.nextafter(mid.float(), torch.full_like(mid.float(), math.inf)).to(DT[dtype])
+    down = torch.nextafter(mid.float(), torch.full_like(mid.float(), -math.inf)).to(DT[dtype])
+    x = torch.cat([mid, up, down], 1).clamp(-top.unsqueeze(1), top.unsqueeze(1)).to(DT[dtype])
+    x = torch.cat([x, top.unsqueeze(1).to(DT[dtype]), -top.unsqueeze(1).to(DT[dtype])], 1)
+    q, sc = quantized(ctx, x.cuda())
+    rq, rs = quantize64(x)
+    assert torch.equal(sc.cpu(), rs) and torch.equal(q.cpu().long(), rq)
 
 
 def test_quantize_leaves_the_padding(ctx):
