@@ -1250,6 +1250,22 @@ class StepOutcome:
         self.consumed_state = next_state
 
 
+class ScoreOutcome:
+    """One sequence's scores: logprobs [n - 1] of its tokens after the first,
+    given those before; entropy [n] in nats, top_ids [n][k] and top_logprobs
+    [n][k] of the distribution behind each token (the last: the next token's)."""
+
+    __slots__ = ("logprobs", "entropy", "top_ids", "top_logprobs")
+
+    def __init__(self, logprobs: np.ndarray, entropy: np.ndarray, top_ids: np.ndarray, top_logprobs: np.ndarray):
+        self.logprobs, self.entropy, self.top_ids, self.top_logprobs = logprobs, entropy, top_ids, top_logprobs
+
+    @classmethod
+    def empty(cls, top: int) -> "ScoreOutcome":
+        f = np.zeros(0, np.float32)
+        return cls(f, f, np.zeros((0, top), np.int32), np.zeros((0, top), np.float32))
+
+
 class CudaMoeServingModel:
     """A BatchStepModel (har/crates/har-serve/src/adapter.rs:28-72) over
     har-cuda: the serving seam's contract with the Q4_K MoE stack on the GPU,
@@ -1258,7 +1274,8 @@ class CudaMoeServingModel:
     One step for a batch of (hidden, token): x = hidden + embed[token]; each
     MoE layer routes x with its f32 router on the device and adds its output
     to x (routed_moe + residual, har-native-qwen35moe.rs:1152-1215); logits =
-    out · x with the LM head (Q4_K or Q6_K) GEMV.  Every sequence of the batch
+    out · x with the LM head: a Q4_K or Q6_K GEMV, or the 8-bit product where
+    `out` is I8Weights.  Every sequence of the batch
     shares each weight read: one routed_moe per layer and one GEMV per step
     for the whole batch.  `next` is the hidden state after the layers (the
     reference's toy MoEModel returns its input state instead; a real model's
@@ -1266,7 +1283,7 @@ class CudaMoeServingModel:
     (the fail-closed rule of vulkan.rs:18-19); nothing falls back to the CPU.
     """
 
-    def __init__(self, ctx: Context, layers, embed: np.ndarray, out: Q4KWeights, k: int,
+    def __init__(self, ctx: Context, layers, embed: np.ndarray, out, k: int,
                  eos: int, routers=None, flags: int = 0):
         import torch
         self.ctx, self.layers, self.k, self._eos, self.flags = ctx, list(layers), k, eos, flags
@@ -1285,23 +1302,31 @@ class CudaMoeServingModel:
         self.last_routes = None  # [(ids [B][k], weights [B][k]) per layer] of the last step
         self.telemetry = {"positions": 0, "expert_reads": 0, "shared_reads": 0}
 
-    def _step_device(self, x):
+    def _layers_device(self, x):
+        """Every layer routed and applied in one library call: (the rows after
+        the last layer, [(ids, weights) per layer])."""
         torch = self._torch
         B, L = x.shape[0], len(self.layers)
-        # every layer routed and applied in one library call
         ids = torch.empty((L, B, self.k), dtype=torch.int32, device=self._dev)
         w = torch.empty((L, B, self.k), dtype=torch.float32, device=self._dev)
         y = torch.empty_like(x)
         self.ctx.routed_moe_stack(self.layers, self.routers, x, self.k, ids, w, y,
                                   self.flags | MOE_ADD_RESIDUAL)
-        routes = [(ids[l], w[l]) for l in range(L)]
-        x = y
-        logits = torch.empty((B, self.vocab), dtype=torch.float32, device=self._dev)
-        if self.out.ggml_type == GGML_Q6_K:
-            self.ctx.q6k_gemv(self.out, 0, x, B, logits)
+        return y, [(ids[l], w[l]) for l in range(L)]
+
+    def _logits_device(self, x):
+        logits = self._torch.empty((x.shape[0], self.vocab), dtype=self._torch.float32, device=self._dev)
+        if isinstance(self.out, I8Weights):
+            self.ctx.i8_linear(self.out, x, logits)
+        elif self.out.ggml_type == GGML_Q6_K:
+            self.ctx.q6k_gemv(self.out, 0, x, x.shape[0], logits)
         else:
-            self.ctx.q4k_gemv(self.out, 0, x, ACT_F32, B, logits)
-        return x, logits, routes
+            self.ctx.q4k_gemv(self.out, 0, x, ACT_F32, x.shape[0], logits)
+        return logits
+
+    def _step_device(self, x):
+        x, routes = self._layers_device(x)
+        return x, self._logits_device(x), routes
 
     def batch_step(self, inputs):
         """BatchStepModel::batch_step: inputs [(hidden [H], token)] ->
@@ -1322,6 +1347,61 @@ class CudaMoeServingModel:
         self.telemetry["expert_reads"] += sum(len(np.unique(i)) for i, _ in self.last_routes)
         self.telemetry["shared_reads"] += len(self.layers)
         return [StepOutcome(nxt[i], lg[i]) for i in range(len(inputs))]
+
+    # rows whose logits are held at a time where the head is block-quantised
+    SCORE_ROWS = 128
+
+    def _score_device(self, x, tokens, top: int):
+        """(logprobs [P], entropy [P], top_ids [P][top], top_logprobs [P][top])
+        for the rows x [P][H] after the layers and the tokens int32 [P] they
+        are asked for (-1: none, 0)."""
+        torch = self._torch
+        P = x.shape[0]
+        f = dict(dtype=torch.float32, device=self._dev)
+        lp, en, tl = torch.empty((P, 1), **f), torch.empty(P, **f), torch.empty((P, top), **f)
+        ti = torch.empty((P, top), dtype=torch.int32, device=self._dev)
+        tok = tokens.reshape(P, 1)
+        if isinstance(self.out, I8Weights):
+            self.ctx.i8_head_logprobs(self.out, x, tok, lp, en, ti, tl)
+        else:
+            for p in range(0, P, self.SCORE_ROWS):
+                r = slice(p, p + self.SCORE_ROWS)
+                self.ctx.token_logprobs(self._logits_device(x[r]), tok[r], lp[r], en[r], ti[r], tl[r])
+        return lp[:, 0], en, ti, tl
+
+    def score(self, inputs, top: int = 0):
+        """Log probabilities of given sequences: inputs [(hidden [H], tokens)]
+        -> [ScoreOutcome], one per input, in order.  The tokens are folded
+        through the layers as prefill_batch folds them, sequences side by side
+        (a row's step does not depend on the others'), and the head is applied
+        once, to every position of the batch: no [positions][vocab] logits with
+        an 8-bit head.  `top` alternatives a position, at most LOGPROBS_MAX_TOP."""
+        torch = self._torch
+        seqs = [np.asarray(t, np.int64).reshape(-1) for _, t in inputs]
+        if not 0 <= top <= LOGPROBS_MAX_TOP:
+            raise HarCudaError(ERR_ARG, f"score: 0 <= top <= {LOGPROBS_MAX_TOP}")
+        for s in seqs:
+            if s.size and (s.min() < 0 or s.max() >= self.vocab):
+                raise HarCudaError(ERR_ARG, "token id outside the vocabulary")
+        P = sum(s.size for s in seqs)
+        if P == 0:
+            return [ScoreOutcome.empty(top) for _ in seqs]
+        at = np.cumsum([0] + [s.size for s in seqs])  # sequence i's positions start at at[i]
+        rows = torch.empty((P, self.H), dtype=torch.float32, device=self._dev)
+        hid = torch.from_numpy(np.stack([np.asarray(h, np.float32).reshape(self.H) for h, _ in inputs])).to(self._dev)
+        for i in range(max(s.size for s in seqs)):
+            live = [j for j, s in enumerate(seqs) if s.size > i]
+            t = torch.from_numpy(np.asarray([seqs[j][i] for j in live])).to(self._dev)
+            prev = hid[live] if i == 0 else rows[torch.from_numpy(at[live] + i - 1).to(self._dev)]
+            y, _ = self._layers_device((prev + self.embed[t]).contiguous())
+            rows[torch.from_numpy(at[live] + i).to(self._dev)] = y
+        nxt = np.full(P, -1, np.int32)
+        for j, s in enumerate(seqs):
+            nxt[at[j]:at[j + 1] - 1] = s[1:]
+        lp, en, ti, tl = self._score_device(rows, torch.from_numpy(nxt).to(self._dev), top)
+        self.ctx.synchronize()
+        lp, en, ti, tl = (v.cpu().numpy() for v in (lp, en, ti, tl))
+        return [ScoreOutcome(lp[a:max(a, b - 1)], en[a:b], ti[a:b], tl[a:b]) for a, b in zip(at[:-1], at[1:])]
 
     def prefill_batch(self, inputs):
         """The trait's default prefill (adapter.rs:42-61): batch_step folded

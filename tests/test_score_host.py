@@ -2,6 +2,7 @@
 null contexts and handles, tensors on the CPU."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -50,3 +51,56 @@ def test_tensors_on_the_cpu_are_refused():
 def test_row_matrix_strides():
     q = har_cuda.i8_rows(3, 33, "cpu")
     assert tuple(q.shape) == (3, 33) and q.stride() == (48, 1)
+
+
+class _Fold(har_cuda.CudaMoeServingModel):
+    """The scoring path with its device steps replaced by torch on the CPU: a
+    layer step halves its row, the head's logits are the row itself."""
+
+    def __init__(self, V):
+        self.H = self.vocab = V
+        self._torch, self._dev = torch, torch.device("cpu")
+        self.embed = torch.eye(V)
+        self.batches, self.ctx = [], type("C", (), {"synchronize": lambda s: None})()
+
+    def _layers_device(self, x):
+        self.batches.append(x.shape[0])
+        return x * 0.5, []
+
+    def _score_device(self, x, tokens, top):
+        logp = torch.log_softmax(x.double(), 1)
+        lp = torch.where(tokens < 0, 0.0, logp.gather(1, tokens.clamp(min=0).long().unsqueeze(1))[:, 0])
+        best = logp.sort(dim=1, descending=True, stable=True)
+        return lp, -(logp.exp() * logp).sum(1), best.indices[:, :top].int(), best.values[:, :top]
+
+
+def test_score_folds_sequences_side_by_side():
+    V = 7
+    m = _Fold(V)
+    rng = np.random.default_rng(1)
+    h = rng.normal(size=(4, V)).astype(np.float32)
+    seqs = [[3, 1, 1, 6], [2], [], [0, 5, 4]]
+    outs = m.score(list(zip(h, seqs)), top=3)
+    assert m.batches == [3, 2, 2, 1]           # sequences that still have a token
+    for i, toks in enumerate(seqs):
+        o, x = outs[i], h[i].astype(np.float64)
+        assert o.logprobs.shape == (max(0, len(toks) - 1),) and o.entropy.shape == (len(toks),)
+        assert o.top_ids.shape == (len(toks), 3) and o.top_logprobs.shape == (len(toks), 3)
+        for j, t in enumerate(toks):
+            x = (x + np.eye(V)[t]) * 0.5
+            logp = x - np.log(np.exp(x).sum())
+            assert np.allclose(o.entropy[j], -(np.exp(logp) * logp).sum(), atol=1e-6)
+            assert o.top_ids[j].tolist() == np.argsort(-logp, kind="stable")[:3].tolist()
+            if j + 1 < len(toks):
+                assert np.allclose(o.logprobs[j], logp[toks[j + 1]], atol=1e-6)
+    assert m.score([]) == []
+    assert [o.entropy.size for o in m.score([(h[0], [])])] == [0]
+
+
+def test_score_refuses():
+    m = _Fold(5)
+    for bad in ([5], [-1]):
+        with pytest.raises(har_cuda.HarCudaError):
+            m.score([(np.zeros(5, np.float32), bad)])
+    with pytest.raises(har_cuda.HarCudaError):
+        m.score([(np.zeros(5, np.float32), [1])], top=33)
