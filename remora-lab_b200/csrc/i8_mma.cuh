@@ -30,12 +30,14 @@ struct Ring {
   int abort_flag;
 };
 
-// What every role knows: K in k-steps, the tile's columns, ring slots.
+// What every role knows: K, the k-steps [k0, k1) of it that a tile takes, the
+// tile's columns, ring slots.
 struct RingShape {
   int64_t K;
+  int k0, k1;
   int bn, stages;
-  __device__ __forceinline__ int ksteps() const { return (int)((K + G_KS - 1) / G_KS); }
 };
+inline int ksteps_of(int64_t K) { return (int)((K + G_KS - 1) / G_KS); }
 
 __device__ __forceinline__ bool g_wait(uint64_t *bar, uint32_t parity, volatile int *abort_s, uint32_t sleep_ns = 0) {
   if (*abort_s) return false;
@@ -118,18 +120,19 @@ template <int CG, typename Tiles>
 __device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8_t *sm, bool is_b, const void *map,
                                              Tiles tiles, uint32_t rank) {
   volatile int *abort_s = &r.abort_flag;
-  const int b_rows = sh.bn / CG, ksteps = sh.ksteps();
+  const int b_rows = sh.bn / CG;
+  const uint32_t even = CG == 2 ? tc::cluster_rank() & ~1u : 0u;
   const uint32_t a_bytes = G_A * G_KS, b_bytes = (uint32_t)b_rows * G_KS, bytes = is_b ? b_bytes : a_bytes;
   uint32_t it = 0;
   int a_row, b_row;
   while (tiles.next(a_row, b_row)) {
     const int row = is_b ? b_row + (int)rank * b_rows : a_row + (int)rank * G_A;
-    for (int k = 0; k < ksteps; ++k, ++it) {
+    for (int k = sh.k0; k < sh.k1; ++k, ++it) {
       const int s = (int)(it % (uint32_t)sh.stages);
       if (!g_wait(r.empty + s, ((it / (uint32_t)sh.stages) & 1u) ^ 1u, abort_s, 64)) return;
       uint8_t *dst = sm + (size_t)s * (a_bytes + b_bytes) + (is_b ? a_bytes : 0);
       if (rank == 0) tc::mbar_expect_tx(r.full + s, CG * bytes);
-      if (CG == 2) tc::tma_load_2d_pair(dst, map, k * G_KS, row, tc::map_rank(tc::smem_u32(r.full + s), 0));
+      if (CG == 2) tc::tma_load_2d_pair(dst, map, k * G_KS, row, tc::map_rank(tc::smem_u32(r.full + s), even));
       else tc::tma_load_2d(dst, map, k * G_KS, row, r.full + s);
     }
   }
@@ -139,11 +142,11 @@ __device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8
 template <int CG, typename Tiles>
 __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t *sm, Tiles tiles) {
   volatile int *abort_s = &r.abort_flag;
-  const int lane = threadIdx.x & 31, ksteps = sh.ksteps();
-  const uint32_t lead = tc::elect_one(), tmem = r.tmem;
+  const int lane = threadIdx.x & 31;
+  const uint32_t lead = tc::elect_one(), tmem = r.tmem, even = CG == 2 ? tc::cluster_rank() : 0u;
   const uint32_t a_bytes = G_A * G_KS, slot = a_bytes + (uint32_t)(sh.bn / CG) * G_KS;
   const uint32_t idesc = tc::idesc_i8(CG * G_A, sh.bn);
-  const int last = (int)((sh.K - (int64_t)(ksteps - 1) * G_KS + 31) / 32);  // MMAs of the last k-step
+  const int tail = (int)((sh.K - (int64_t)(sh.k1 - 1) * G_KS + 31) / 32);  // MMAs of the last k-step
   uint32_t it = 0;
   int a_row, b_row;
   for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
@@ -161,23 +164,23 @@ __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t
     }
     tc::tc_fence_after();
     const uint32_t d = tmem + a * 256u;
-    for (int k = 0; k < ksteps; ++k, ++it) {
+    for (int k = sh.k0; k < sh.k1; ++k, ++it) {
       const int s = (int)(it % (uint32_t)sh.stages);
       if (!g_wait_warp(r.full + s, (it / (uint32_t)sh.stages) & 1u, abort_s, lane)) return;
       tc::tc_fence_after();
       const uint32_t base = tc::smem_u32(sm + (size_t)s * slot);
       const uint64_t ad = tc::desc_sw128(base), bd = tc::desc_sw128(base + a_bytes);
-      const int slices = k == ksteps - 1 ? last : 4;
+      const int slices = k == sh.k1 - 1 ? min(tail, 4) : 4;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (j < slices) {
-          if (CG == 2) tc::mma_i8_pair_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, (k | j) ? 1u : 0u);
-          else tc::mma_i8_ss_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, (k | j) ? 1u : 0u);
+          if (CG == 2) tc::mma_i8_pair_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, k != sh.k0 || j ? 1u : 0u);
+          else tc::mma_i8_ss_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, k != sh.k0 || j ? 1u : 0u);
         }
-      if (CG == 2) tc::mma_commit_pair_w(lead, r.empty + s);
+      if (CG == 2) tc::mma_commit_pair_w(lead, r.empty + s, even);
       else tc::mma_commit_w(lead, r.empty + s);
     }
-    if (CG == 2) tc::mma_commit_pair_w(lead, r.acc_full + a);
+    if (CG == 2) tc::mma_commit_pair_w(lead, r.acc_full + a, even);
     else tc::mma_commit_w(lead, r.acc_full + a);
   }
 }
@@ -188,7 +191,7 @@ __device__ __forceinline__ void ring_release(Ring &r, uint32_t a, int lane) {
   tc::tc_fence_before();
   __syncwarp();
   if (lane == 0) {
-    if (CG == 2) tc::mbar_arrive_cluster(tc::map_rank(tc::smem_u32(r.acc_empty + a), 0));
+    if (CG == 2) tc::mbar_arrive_cluster(tc::map_rank(tc::smem_u32(r.acc_empty + a), tc::cluster_rank() & ~1u));
     else tc::mbar_arrive(r.acc_empty + a);
   }
 }

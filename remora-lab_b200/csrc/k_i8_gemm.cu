@@ -195,38 +195,142 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   ring_close<CG>(ring, p.status);
 }
 
-// Blocks a tile and tokens of a tile: the split of M into equal tiles that
-// costs least.  A k-step of a tile costs a lone block its MMAs (2 cycles a
-// token at 8,192 products a cycle) or its bytes from L2 (about 42 a cycle
-// measured, with all blocks loading), whichever is more; a pair moves half the
-// token bytes.  A tile costs about 1,500 cycles to fill and drain, a pair 500
-// more to join.
-static int pick_tile(int64_t M, int64_t N, int64_t K, int sms, int &cg) {
-  const int64_t ksteps = (K + G_KS - 1) / G_KS;
-  double best = 0;
-  int bn = 0;
-  for (int g = 1; g <= 2; ++g) {
-    const int64_t nt = (N + g * G_A - 1) / (g * G_A), first = (M + G_MAX_BN - 1) / G_MAX_BN;
-    for (int64_t mt = first; mt <= first + 15; ++mt) {
-      const int64_t b = ((M + mt - 1) / mt + 16 * g - 1) / (16 * g) * (16 * g);
-      const int64_t tiles = nt * ((M + b - 1) / b), waves = (tiles + sms / g - 1) / (sms / g);
-      const double bytes = G_A * G_KS + b / g * G_KS;
-      const double cost = waves * (ksteps * std::max(2.0 * b, bytes / 42.0) + 1500.0 + 500.0 * (g - 1));
-      if (!bn || cost < best) best = cost, bn = (int)b, cg = g;
+// The same product where there are fewer tiles than pairs: a cluster of S pairs
+// shares one tile, each pair a part of K, because a block alone brings in no
+// more than about 65 GB/s (512 x 2048 x 2048: 16 k-steps took 5.1 us whatever
+// the tile's size).  The pairs leave their 32-bit sums in their shared memory;
+// pair s reads every pair's sums of token slice s, adds them up (whole numbers:
+// any order) and writes its slice.  (Sent instead of fetched they took two
+// barriers and 3.3 us for the smallest tile.)
+template <typename T, int S>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    i8_split_kernel(const __grid_constant__ TmaDesc map_w, const __grid_constant__ TmaDesc map_x, GemmParams p) {
+  extern __shared__ uint8_t g_raw[];
+  __shared__ Ring ring;
+  uint8_t *sm = g_raw + ((1024u - (tc::smem_u32(g_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = tc::cluster_rank(), rank = crank & 1u, part = crank >> 1;
+  const int all = p.sh.k1;  // at least 2 S, so no part is empty
+  p.sh.k0 = all * (int)part / S;
+  p.sh.k1 = all * ((int)part + 1) / S;
+  // this cluster's tile, once
+  struct One {
+    int a_row, b_row;
+    bool left;
+    __device__ __forceinline__ bool next(int &a, int &b) {
+      a = a_row, b = b_row;
+      const bool was = left;
+      left = false;
+      return was;
+    }
+  };
+  const int tile = (int)(blockIdx.x / (2 * S));
+  const One one = {tile / p.mt * (2 * G_A), tile % p.mt * p.sh.bn, true};
+  ring_open<2>(ring, p.sh, &map_w, &map_x);
+
+  const int quad = warp & 3, h = (warp - G_WARP_EPI) >> 2;
+  const int half = (p.sh.bn / 16 + 1) / 2 * 16, slice = p.sh.bn / S;
+  const int cols = h == 0 ? half : p.sh.bn - half;  // this half's tokens
+  uint32_t v[4][32];
+  bool ok = false;
+  if (warp == G_WARP_A) {
+    if (lane == 0) ring_produce<2>(ring, p.sh, sm, false, &map_w, one, rank);
+  } else if (warp == G_WARP_B) {
+    if (lane == 0) ring_produce<2>(ring, p.sh, sm, true, &map_x, one, rank);
+  } else if (warp == G_WARP_MMA) {
+    if (rank == 0) ring_issue<2>(ring, p.sh, sm, one);
+  } else {
+    ok = g_wait_warp(ring.acc_full, 0, &ring.abort_flag, lane, 64);
+    tc::tc_fence_after();
+    const uint32_t col = ring.tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(h * half);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (ok && 32 * j < cols) tc::tmem_ld32(col + (uint32_t)(32 * j), v[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tc::tmem_wait_ld32(v[j]);
+  }
+  if (warp >= G_WARP_EPI && ok) {
+    // the pair's MMAs are done with the ring: it takes the sums, [token][128 channels]
+    uint32_t *mine = reinterpret_cast<uint32_t *>(sm) + (h * half) * G_A + 32 * quad + lane;
+#pragma unroll
+    for (int c = 0; c < 128; ++c)
+      if (c < cols) mine[c * G_A] = v[c >> 5][c & 31];
+  }
+  __syncwarp();
+  tc::cluster_arrive();
+  tc::cluster_wait();
+  if (warp >= G_WARP_EPI) {
+    const int tid = (int)threadIdx.x - 32 * G_WARP_EPI, c = 4 * (tid & 31);
+    const int64_t chan = (int64_t)one.a_row + rank * G_A + c, m0 = (int64_t)one.b_row + part * slice;
+    const int tokens = (int)max((int64_t)0, min((int64_t)slice, p.M - m0));
+    const int chans = (int)max((int64_t)0, min((int64_t)4, p.N - chan));
+    float sw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sw[i] = i < chans ? __ldg(p.sw + chan + i) : 0.0f;
+    uint32_t from[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      from[s] = tc::map_rank(tc::smem_u32(sm) + ((uint32_t)(part * slice) * G_A + (uint32_t)c) * 4u, (uint32_t)(2 * s) + rank);
+#pragma unroll 2
+    for (int t = tid >> 5; t < tokens; t += G_EPI_WARPS) {
+      int4 a[S];
+#pragma unroll
+      for (int s = 0; s < S; ++s) a[s] = tc::ld_cluster_v4(from[s] + (uint32_t)t * (G_A * 4u));
+#pragma unroll
+      for (int s = 1; s < S; ++s) a[0].x += a[s].x, a[0].y += a[s].y, a[0].z += a[s].z, a[0].w += a[s].w;
+      const float sx = __ldg(p.sx + m0 + t);
+      const int sum[4] = {a[0].x, a[0].y, a[0].z, a[0].w};
+      T *y = (T *)p.y + (m0 + t) * p.ldy + chan;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < chans) y[i] = from_f32<T>(__fmul_rn(__int2float_rn(sum[i]), __fmul_rn(sx, sw[i])));
     }
   }
-  return bn;
+  ring_close<2>(ring, p.status);
+}
+
+// How a product is cut up.  Blocks a tile (cg), tokens of a tile (bn), pairs
+// that share a tile (split): the cheapest by these measures.  A k-step of a
+// tile costs a lone block its MMAs (2 cycles a token at 8,192 products a cycle)
+// or its bytes from L2 (about 42 a cycle measured, with all blocks loading) or
+// 540 cycles, the time a box of 128 rows takes at the least; a pair moves half
+// the token bytes.  A tile costs about 1,500 cycles to fill and drain, a pair
+// 500 more to join, and 2,500 if its sums have to meet.  Clusters of 4 and 8
+// blocks do not fill every group of SMs: 35 and 15 of them ran at a time.
+struct GemmPlan {
+  int cg, bn, split;
+};
+static GemmPlan pick_plan(int64_t M, int64_t N, int64_t K, int sms) {
+  const int64_t ksteps = ksteps_of(K), first = (M + G_MAX_BN - 1) / G_MAX_BN;
+  double best = 0;
+  GemmPlan plan = {};
+  for (int g = 1; g <= 2; ++g) {
+    const int64_t nt = (N + g * G_A - 1) / (g * G_A);
+    for (int64_t mt = first; mt <= first + 15; ++mt) {
+      const int64_t b = ((M + mt - 1) / mt + 16 * g - 1) / (16 * g) * (16 * g);
+      const int64_t tiles = nt * ((M + b - 1) / b);
+      const double step = std::max({2.0 * b, (G_A * G_KS + b / g * G_KS) / 42.0, 540.0});
+      for (int s = 1; s <= (g == 2 ? 4 : 1); s *= 2) {
+        if (s > 1 && (tiles > (s == 2 ? 35 : 15) * sms / 148 || ksteps < 2 * s)) continue;
+        const int64_t waves = (tiles * s + sms / g - 1) / (sms / g);
+        const double cost = waves * ((ksteps + s - 1) / s * step + 1500.0 + 500.0 * (g - 1)) + (s > 1 ? 2500.0 : 0.0);
+        if (!plan.bn || cost < best) best = cost, plan = {g, (int)b, s};
+      }
+    }
+  }
+  return plan;
 }
 
 int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q,
                          int64_t ldq, const float *scale, int64_t M, void *y, int32_t y_dtype,
                          int64_t ldy) {
+  const GemmPlan plan = pick_plan(M, w->N, w->K, ctx->num_sms);
+  const int cg = plan.cg;
   GemmParams p = {};
-  int cg = 1;
   p.M = M, p.N = w->N, p.ldy = ldy;
   p.sx = scale, p.sw = w->scale, p.y = y, p.status = ctx->d_status;
-  p.sh.K = w->K;
-  p.sh.bn = pick_tile(M, w->N, w->K, ctx->num_sms, cg);
+  p.sh.K = w->K, p.sh.k0 = 0, p.sh.k1 = ksteps_of(w->K);
+  p.sh.bn = plan.bn;
   p.sh.stages = cg == 2 ? ring_stages<2>(p.sh.bn) : ring_stages<1>(p.sh.bn);
   p.mt = (int)((M + p.sh.bn - 1) / p.sh.bn);
   p.nt = (int)((w->N + cg * G_A - 1) / (cg * G_A));
@@ -237,24 +341,29 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
   // store fills the last 16 bytes of a row with zeros)
   TmaDesc map_y = map_x;
   const size_t eb = dtype_bytes(y_dtype);
-  p.store = ((uintptr_t)y & 15u) == 0 && (w->N * (int64_t)eb) % 16 == 0 && (M == 1 || (ldy * (int64_t)eb) % 16 == 0);
+  p.store = plan.split == 1 && ((uintptr_t)y & 15u) == 0 && (w->N * (int64_t)eb) % 16 == 0 &&
+            (M == 1 || (ldy * (int64_t)eb) % 16 == 0);
   if (p.store) {
     const uint64_t pitch = (uint64_t)(M == 1 ? w->N : ldy) * eb;
     st = encode_tmap_2d(ctx, &map_y, y, (int)eb, (uint64_t)M, (uint64_t)w->N, pitch, 16, G_A, false);
     if (st != HAR_CUDA_OK) return st;
   }
   const unsigned grid = (unsigned)std::min<int64_t>(ctx->num_sms / cg, (int64_t)p.mt * p.nt) * cg;
+  const unsigned split_grid = (unsigned)(p.mt * p.nt * 2 * plan.split);
   cudaError_t e = cudaSuccess;
+  const char *name = plan.split > 1 ? "i8_split_kernel" : "i8_gemm_kernel";
   prof_begin(ctx);
   with_dtype(y_dtype, [&](auto t) {
     using T = decltype(t);
-    const size_t smem = G_STAGE_BYTES + G_SLABS * G_SLAB + 1024;
-    e = cg == 2 ? launch_clusters(i8_gemm_kernel<T, 2>, grid, G_THREADS, smem, ctx->stream, 2, w->map, map_x, map_y, p)
-                : launch_clusters(i8_gemm_kernel<T, 1>, grid, G_THREADS, smem, ctx->stream, 1, w->map, map_x, map_y, p);
+    const size_t smem = G_STAGE_BYTES + G_SLABS * G_SLAB + 1024, split_smem = G_STAGE_BYTES + 1024;
+    e = plan.split == 4 ? launch_clusters(i8_split_kernel<T, 4>, split_grid, G_THREADS, split_smem, ctx->stream, 8, w->map, map_x, p)
+        : plan.split == 2 ? launch_clusters(i8_split_kernel<T, 2>, split_grid, G_THREADS, split_smem, ctx->stream, 4, w->map, map_x, p)
+        : cg == 2 ? launch_clusters(i8_gemm_kernel<T, 2>, grid, G_THREADS, smem, ctx->stream, 2, w->map, map_x, map_y, p)
+                  : launch_clusters(i8_gemm_kernel<T, 1>, grid, G_THREADS, smem, ctx->stream, 1, w->map, map_x, map_y, p);
   });
-  st = check_launch(ctx, "i8_gemm_kernel");
+  st = check_launch(ctx, name);
   if (e != cudaSuccess)
-    return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_gemm_kernel: ") + cudaGetErrorString(e));
+    return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string(name) + ": " + cudaGetErrorString(e));
   return st;
 }
 

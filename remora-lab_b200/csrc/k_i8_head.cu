@@ -553,7 +553,7 @@ int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     const uint8_t *xs = (const uint8_t *)x + (size_t)(t0 * ldx) * dtype_bytes(x_dtype);
     int32_t st = launch_i8_quantize(ctx, xs, x_dtype, n, w->K, ldx, q, ldq, sx);
     if (st != HAR_CUDA_OK) return st;
-    p.sh.K = w->K;
+    p.sh.K = w->K, p.sh.k0 = 0, p.sh.k1 = ksteps_of(w->K);
     p.sh.bn = H_TILE;
     const int cap = k > H_LONG ? H_CAP_LONG : H_CAP;
     p.sh.stages = k > H_LONG ? H_SLOTS_LONG : H_SLOTS;

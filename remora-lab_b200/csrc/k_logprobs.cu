@@ -9,7 +9,7 @@ namespace har {
 
 namespace cg = cooperative_groups;
 
-constexpr int LP_T = 256, LP_WARPS = LP_T / 32, LP_U = 4, LP_SEG = 32, LP_MAX_CLUSTER = 16;
+constexpr int LP_U = 4, LP_MAX_CLUSTER = 16;
 constexpr int LP_QUEUE = 256, LP_CAND = 512;
 // One 16-byte piece of a row.
 template <typename T>
@@ -56,18 +56,19 @@ __device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
 }
 
 // A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
-// part of its pieces, walked in trips of LP_T x LP_U pieces.  The alternatives
+// part of its pieces, walked in trips of LP_T (its threads) x LP_U pieces.  The alternatives
 // cost the walk one store: a thread notes the largest element of each trip (a
-// group of LP_U pieces).  After up to LP_SEG trips a bound is taken that at
+// group of LP_U pieces).  After some trips (LP_SEG) a bound is taken that at
 // least k of the threads' largest elements reach, so only groups that reach it
 // (k or a few more of thousands) can hold an alternative: they are queued, read
 // again from L2, one element a lane, and the elements that reach the bound are
 // sorted.  Where ties are so many that the queue overflows, each warp goes
 // through its own groups in order instead.
-template <typename T>
-__global__ void __launch_bounds__(LP_T, 4)
+template <typename T, int LP_T>
+__global__ void __launch_bounds__(LP_T, 1024 / LP_T)
     token_logprobs_kernel(const T *__restrict__ logits, int64_t V, int64_t ldl, LogprobOut out, int C) {
-  constexpr int N = Piece<T>::N;
+  constexpr int N = Piece<T>::N, LP_WARPS = LP_T / 32;
+  constexpr int LP_SEG = LP_T == 256 ? 32 : 40;  // trips between two searches
   __shared__ float group_top[LP_SEG][LP_T];
   __shared__ uint32_t warp_top[LP_WARPS], least_s;
   __shared__ int queued, found;
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(LP_T, 4)
       stat_add<LP_U * N>(st, top, [&](int i) { return p[i / N].at(i % N); });
     }
     if (!want_top) continue;
-    // each warp's ceil(k / 8)-th largest thread: together at least k elements
-    // reach the smallest of the eight
+    // each warp's ceil(k / warps)-th largest thread: together at least k elements
+    // reach the smallest of these
     const uint32_t sorted = warp_sort_desc(order_bits(most), lane);
     if (lane == (out.k + LP_WARPS - 1) / LP_WARPS - 1) warp_top[warp] = sorted;
     __syncthreads();
@@ -276,9 +277,9 @@ __global__ void __launch_bounds__(LP_T, 4)
   }
 }
 
-// Blocks a row: 1 to 16, a power of two.  4 blocks an SM run at a time; one
-// takes about 5 us to start, to find its alternatives and to join, and reads
-// 16 KB/us alone or beside another, 11 beside three.
+// Blocks a row: 1 to 16, a power of two.  1,024 threads an SM run at a time; a
+// block takes about 5 us to start, to find its alternatives and to join, and
+// one of 256 threads reads 16 KB/us alone or beside another, 11 beside three.
 static int pick_cluster(int64_t T, int64_t bytes, int sms) {
   int best = 1;
   double least = 0;
@@ -308,11 +309,15 @@ int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dty
     prof_begin(ctx);
     with_dtype(dtype, [&](auto t) {
       using E = decltype(t);
-      if (C > 8) e = cudaFuncSetAttribute(token_logprobs_kernel<E>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      // many rows, not the longest: blocks of 128 threads, so that more rows are
+      // in different phases and the ends of some overlap the walks of others
+      // (4,096 rows of 5,000 f32: 57 -> 40 us; 2,048 of 131,072 f32: 185 -> 196)
+      const bool narrow = C == 1 && T >= 8 * ctx->num_sms && V * (int64_t)sizeof(E) <= 384 * 1024;
+      if (C > 8) e = cudaFuncSetAttribute(token_logprobs_kernel<E, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(rows * C));
-      cfg.blockDim = dim3(LP_T);
+      cfg.blockDim = dim3(narrow ? 128 : 256);
       cfg.stream = ctx->stream;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -320,7 +325,8 @@ int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dty
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = C > 1 ? 1 : 0;
-      e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<E>, (const E *)logits + t0 * ldl, V, ldl, o, C);
+      e = cudaLaunchKernelEx(&cfg, narrow ? token_logprobs_kernel<E, 128> : token_logprobs_kernel<E, 256>,
+                             (const E *)logits + t0 * ldl, V, ldl, o, C);
     });
     const int32_t st = check_launch(ctx, "token_logprobs_kernel");
     if (e != cudaSuccess)

@@ -70,7 +70,7 @@ __device__ __forceinline__ void stat_add(Stat &a, float top, At &&at) {
   if (top > a.r + 6.0f) stat_move(a, top);
   const float r = a.r == -INFINITY ? 0.0f : a.r;
   const float2 nr = make_float2(-r, -r), l2e = make_float2(LOG2E, LOG2E);
-  float2 s = make_float2(a.s, 0.0f), t = make_float2(a.t, 0.0f);
+  float2 s = make_float2(0.0f, 0.0f), t = s;  // added to the row's sums once: fewer roundings at their size
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     float2 d = __fadd2_rn(make_float2(at(i), at(i + 1)), nr);
@@ -81,8 +81,8 @@ __device__ __forceinline__ void stat_add(Stat &a, float top, At &&at) {
     s = __fadd2_rn(s, e);
     t = __ffma2_rn(e, d, t);
   }
-  a.s = s.x + s.y;
-  a.t = t.x + t.y;
+  a.s += s.x + s.y;
+  a.t += t.x + t.y;
 }
 
 }  // namespace har

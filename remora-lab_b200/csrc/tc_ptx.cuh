@@ -260,6 +260,14 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t a, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
   return r;
 }
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 // Arrives on a barrier of any CTA of the cluster (a mapped address).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -306,15 +314,15 @@ __device__ __forceinline__ void mma_i8_pair_w(uint32_t lead, uint32_t d_tmem, ui
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
       : "memory");
 }
-// Arrives once on the barrier at this offset of both CTAs when every MMA
-// issued so far has completed.
-__device__ __forceinline__ void mma_commit_pair_w(uint32_t lead, uint64_t *bar) {
+// Arrives once on the barrier at this offset of both CTAs of the pair whose
+// even rank is `even`, when every MMA issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair_w(uint32_t lead, uint64_t *bar, uint32_t even) {
   asm volatile(
       "{\n\t.reg .pred e;\n\t"
       "setp.ne.b32 e, %1, 0;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
           smem_u32(bar)),
-      "r"(lead), "h"((uint16_t)3)
+      "r"(lead), "h"((uint16_t)(3u << even))
       : "memory");
 }
 

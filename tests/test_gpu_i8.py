@@ -112,7 +112,8 @@ def test_quantize_leaves_the_padding(ctx):
 SHAPES = [(1, 1, 1), (1, 3, 16), (1, 130, 2048), (2, 64, 15), (3, 127, 17), (4, 1000, 2051), (7, 129, 64),
           (8, 257, 128), (9, 33, 144), (15, 128, 256), (16, 300, 63), (17, 255, 129), (31, 1000, 512),
           (33, 513, 1040), (64, 128, 2048), (65, 140, 300), (128, 384, 1000), (129, 640, 96), (256, 129, 272),
-          (257, 256, 4096), (300, 1031, 777), (513, 260, 1024), (700, 5, 33), (1025, 515, 160), (2050, 1300, 720), (513, 5003, 96), (4100, 300, 48)]
+          (257, 256, 4096), (300, 1031, 777), (513, 260, 1024), (700, 5, 33), (1025, 515, 160), (2050, 1300, 720), (513, 5003, 96), (4100, 300, 48), (16, 1000, 2048),
+          (100, 700, 1153), (512, 1500, 1100), (40, 3000, 600)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
