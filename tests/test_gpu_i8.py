@@ -311,3 +311,46 @@ def test_on_another_stream_and_device_order(ctx):
         ctx.bind_torch_stream()
     rq, rs = quantize64(x * 2)
     assert torch.equal(out.cpu(), product(rq, rs, wq, ws, torch.float32))
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_weights_past_two_gigabytes(ctx, M):
+    """Offsets past 2^31 in the weights and in y."""
+    N, K = 1100003, 2048
+    q = torch.randint(-127, 128, (N, K), dtype=torch.int8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    s = torch.rand(N, device="cuda") * 0.01
+    w = ctx.wrap_i8(q, s)
+    x = rows(71, M, K)
+    pad = 60_000_000 if M > 1 else 0               # rows of y far apart: the last starts past 2^31
+    y = torch.empty(M, N + pad, dtype=torch.float16, device="cuda")[:, :N]
+    ctx.i8_linear(w, x, y)
+    rq, rs = quantize64(x)
+    for a, b in ((0, 300), (N // 2, N // 2 + 300), (N - 300, N)):
+        assert torch.equal(y[:, a:b].cpu(), product(rq, rs, q[a:b], s[a:b], torch.float16)), (a, b)
+
+
+def test_one_workspace_for_two_graphs_in_turn(ctx):
+    """Two captured calls that share a workspace, replayed one after the other
+    on one stream, keep to their own inputs and outputs."""
+    w, wq, ws = weights(ctx, 81, 300, 256)
+    xs = [rows(82 + i, 20 + 30 * i, 256) for i in range(2)]
+    ys = [torch.empty(x.shape[0], 300, device="cuda") for x in xs]
+    work = torch.empty(max(w.linear_workspace(x.shape[0]) for x in xs), dtype=torch.uint8, device="cuda")
+    graphs, side = [], torch.cuda.Stream()
+    try:
+        for x, y in zip(xs, ys):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(side):
+                g.capture_begin()
+                ctx.bind_torch_stream()
+                ctx.i8_linear(w, x, y, workspace=work)
+                g.capture_end()
+            graphs.append(g)
+    finally:
+        ctx.bind_torch_stream()
+    for i in (0, 1, 1, 0, 1):
+        xs[i].mul_(-1.25)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        rq, rs = quantize64(xs[i])
+        assert torch.equal(ys[i].cpu(), product(rq, rs, wq, ws, torch.float32)), i

@@ -292,3 +292,67 @@ def test_rows_of_a_few_values_that_are_not_numbers(ctx, dtype):
         x[2, V // 2] = math.nan
         tok = given(1, 4, V, 1)
         check_logprobs(score(ctx, x, tok, 32), logprobs64(x, tok, 32), (dtype, V))
+
+
+@pytest.mark.parametrize("dtype,T,V,k", [("f32", 600, 300001, 20), ("f32", 1200, 98001, 5), ("f16", 1200, 190001, 32),
+                                         ("bf16", 20000, 131072, 3)])
+def test_long_rows_and_large_matrices(ctx, dtype, T, V, k):
+    """Rows that are searched in several parts, and offsets past 2^31 (the last:
+    2.6e9 logits): rows checked one by one, from both ends."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.empty(T, V, dtype=DT[dtype], device="cuda")
+    for t in range(0, T, 500):
+        x[t:t + 500] = torch.randn(min(500, T - t), V, device="cuda", generator=g) * 2.5
+    x[1, : V - 40] = -math.inf
+    x[T - 2] = x[T - 2].sort().values          # ascending: every part is better than the last
+    x[T - 1] = 1.25
+    tok = given(2, T, V, 1)
+    got = score(ctx, x, tok, k)
+    rows = [0, 1, T // 2, T - 2, T - 1]
+    check_logprobs({n: v[rows] for n, v in got.items()}, logprobs64(x[rows], tok[rows], k), (dtype, T, V))
+
+
+@pytest.mark.parametrize("T,V,K,k", [(200, 1, 16, 1), (200, 33, 48, 32), (140, 300, 80, 32), (300, 257, 640, 24),
+                                     (1000, 600, 64, 5)])
+def test_head_of_few_rows(ctx, T, V, K, k):
+    """More alternatives than vocabulary, tiles that end early, all above 128
+    tokens."""
+    w, q, s = head_of(ctx, V, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(V)).cuda()
+    tok = given(3, T, V, 2)
+    got = head_score(ctx, w, x, tok, k)
+    ctx.synchronize()
+    check_logprobs(got, logprobs64(product(*quantize64(x), q, s, torch.float32), tok, k), (T, V))
+
+
+def test_head_in_several_launches(ctx):
+    """More tokens than one launch takes (4,096): the parts' sizes differ."""
+    T, V, K, k = 9001, 700, 64, 6
+    w, q, s = head_of(ctx, 4, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(5)).cuda()
+    tok = given(6, T, V, 1)
+    got = head_score(ctx, w, x, tok, k)
+    ctx.synchronize()
+    rows = list(range(0, 3)) + list(range(2900, 3300)) + list(range(T - 500, T))
+    ref = logprobs64(product(*quantize64(x[rows]), q, s, torch.float32), tok[rows], k)
+    check_logprobs({n: v[rows] for n, v in got.items()}, ref, T)
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_head_scales_that_are_not_numbers(ctx, T):
+    """Channels whose scale is NaN or overflows: NaN and infinite logits make
+    every value NaN, and the ids still stand in order."""
+    V, K = 300, 32
+    w, q, s = head_of(ctx, 6, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(7)).cuda()
+    tok = given(8, T, V, 1)
+    for bad in ("nan", "big"):
+        s2 = s.clone()
+        if bad == "nan":
+            s2[5:290] = math.nan
+        else:
+            s2[3:295] = 3e38
+        wb = ctx.wrap_i8(q, s2)
+        got = head_score(ctx, wb, x, tok, 32)
+        ctx.synchronize()
+        check_logprobs(got, logprobs64(product(*quantize64(x), q, s2, torch.float32), tok, 32), (bad, T))
