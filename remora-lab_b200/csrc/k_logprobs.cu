@@ -58,23 +58,25 @@ __device__ __forceinline__ float Piece<__nv_bfloat16>::top() const {
 // A cluster of C blocks shares a row (C = 1: no cluster), each a contiguous
 // part of its pieces, walked in trips of LP_T (its threads) x LP_U pieces.  The alternatives
 // cost the walk one store: a thread notes the largest element of each trip (a
-// group of LP_U pieces).  After some trips (LP_SEG) a bound is taken that at
-// least k of the threads' largest elements reach, so only groups that reach it
-// (k or a few more of thousands) can hold an alternative: they are queued, read
-// again from L2, one element a lane, and the elements that reach the bound are
-// sorted.  Where ties are so many that the queue overflows, each warp goes
-// through its own groups in order instead.
+// group of LP_U pieces).  After some trips (LP_SEG) the k-th largest of 32 of
+// the threads' largest elements bounds the k-th largest of all from below, so
+// only groups that reach it (k or a few more of thousands) can hold an
+// alternative: they are queued, read again from L2, one element a lane, and the
+// elements that reach the bound are ranked by counting.
+// Where ties are so many that the queue overflows, each warp goes through its
+// own groups in order instead.
 template <typename T, int LP_T>
 __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
     token_logprobs_kernel(const T *__restrict__ logits, int64_t V, int64_t ldl, LogprobOut out, int C) {
   constexpr int N = Piece<T>::N, LP_WARPS = LP_T / 32;
   constexpr int LP_SEG = LP_T == 256 ? 32 : 40;  // trips between two searches
   __shared__ float group_top[LP_SEG][LP_T];
-  __shared__ uint32_t warp_top[LP_WARPS], least_s;
+  __shared__ uint32_t tops[32], least_s;
   __shared__ int queued, found;
   __shared__ int queue[LP_QUEUE];
   __shared__ key_t cand[LP_CAND];
-  __shared__ key_t lists[LP_MAX_CLUSTER][32];  // the block's lists, then the cluster's
+  __shared__ key_t sorted[32];                 // the block's largest so far
+  __shared__ key_t lists[LP_MAX_CLUSTER][32];  // the cluster's
   __shared__ key_t part_list[LP_WARPS][32];
   __shared__ Stat stats[LP_WARPS], part_stats[LP_MAX_CLUSTER];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -112,8 +114,8 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
     }
   };
   Stat st = {-INFINITY, 0.0f, 0.0f};
-  key_t best = 0;  // warp 0: the row's largest so far
   if (tid == 0) queued = found = 0, least_s = order_bits(-INFINITY) + 1u;  // -inf never enters: see the end
+  if (tid < 32) sorted[tid] = 0;
   Piece<T> next[LP_U];
   if (j0 < j1) load_trip(next, j0);
   for (int64_t seg = j0; seg < j1; seg += (int64_t)LP_SEG * LP_T * LP_U) {
@@ -133,23 +135,23 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
       stat_add<LP_U * N>(st, top, [&](int i) { return p[i / N].at(i % N); });
     }
     if (!want_top) continue;
-    // each warp's ceil(k / warps)-th largest thread: together at least k elements
-    // reach the smallest of these
-    const uint32_t sorted = warp_sort_desc(order_bits(most), lane);
-    if (lane == (out.k + LP_WARPS - 1) / LP_WARPS - 1) warp_top[warp] = sorted;
+    // The k-th largest of 32 of the threads' largest, the best of each warp.
+    // (The exact k-th of all, by counting, cost 2,600 cycles.)
+    constexpr int EACH = 32 / LP_WARPS;
+    const uint32_t mine = order_bits(most), ranked = warp_sort_desc(mine, lane);
+    if (lane < EACH) tops[EACH * warp + lane] = ranked;
     __syncthreads();
-    uint32_t bound = warp_top[0];
-#pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) bound = min(bound, warp_top[w]);
-    bound = max(bound, least_s);
-    if (order_bits(most) >= bound) {
-#pragma unroll 8
+    const uint32_t bound = max(__shfl_sync(0xffffffffu, warp_sort_desc(tops[lane], lane), out.k - 1), least_s);
+    if (mine >= bound) {
+#pragma unroll 4
       for (int s = 0; s < trips; ++s)
         if (order_bits(group_top[s][tid]) >= bound) {
           const int at = atomicAdd(&queued, 1);
           if (at < LP_QUEUE) queue[at] = s * LP_T + tid;
         }
     }
+    // what the parts before had joins the new candidates
+    if (tid < 32 && sorted[tid]) cand[atomicAdd(&found, 1)] = sorted[tid];
     __syncthreads();
     const int nq = queued;
     // element `lane` of a group, -inf outside the row
@@ -167,24 +169,43 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
           v[u] = -INFINITY;
           if (i + u * LP_WARPS < nq) v[u] = element(queue[i + u * LP_WARPS], e[u]);
         }
+        uint32_t in[4];
+        int total = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (order_bits(v[u]) >= bound) {
-            const int at = atomicAdd(&found, 1);
-            if (at < LP_CAND) cand[at] = order_key(v[u], (uint32_t)e[u]);
-          }
+        for (int u = 0; u < 4; ++u) {
+          in[u] = __ballot_sync(0xffffffffu, order_bits(v[u]) >= bound);
+          total += __popc(in[u]);
+        }
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&found, total);
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(in[0] & ((1u << lane) - 1u));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (((in[u] >> lane) & 1u) && at < LP_CAND) cand[at] = order_key(v[u], (uint32_t)e[u]);
+          if (u < 3) at += __popc(in[u] >> lane) + __popc(in[u + 1] & ((1u << lane) - 1u));
+        }
       }
     }
     __syncthreads();
     const int n = found;
-    key_t list = 0;
     if (nq <= LP_QUEUE && n <= LP_CAND) {
-      // up to 64: one warp; more: all
-      for (int i = 32 * warp; i < n; i += n <= 64 ? 32 : LP_T) {
-        if (n <= 64 && warp > 0) break;
-        list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? cand[i + lane] : (key_t)0, lane), lane);
+      if (seg > j0) {
+        if (tid < 32) sorted[tid] = 0;
+        __syncthreads();
+      }
+      if (n <= 64) {
+        block_rank(cand, n, sorted, tid, LP_T);
+      } else {
+        key_t list = 0;
+        for (int i = 32 * warp; i < n; i += LP_T)
+          list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? cand[i + lane] : (key_t)0, lane), lane);
+        part_list[warp][lane] = list;
+        __syncthreads();
+        list = block_merge_lists(part_list, LP_WARPS, warp, lane);
+        if (warp == 0) sorted[lane] = list;
       }
     } else {
+      key_t list = 0;
       float bar = -INFINITY;  // the k-th entry's value, once there are k
       for (int s = 0; s < trips; ++s) {
         const float top = group_top[s][tid];
@@ -202,20 +223,17 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
         const key_t last = __shfl_sync(0xffffffffu, list, out.k - 1);
         if (last) bar = order_value((uint32_t)(last >> 32));
       }
-    }
-    if (nq > LP_QUEUE || n > 64) {
       part_list[warp][lane] = list;
       __syncthreads();
       list = block_merge_lists(part_list, LP_WARPS, warp, lane);
+      if (warp == 0) sorted[lane] = warp_merge_desc(list, sorted[lane], lane);
     }
-    if (warp == 0) {
-      best = seg == j0 ? list : warp_merge_desc(best, list, lane);
+    __syncthreads();
+    if (tid == 0) {
       // what comes later and only equals the k-th entry loses to it
-      const key_t last = __shfl_sync(0xffffffffu, best, out.k - 1);
-      if (lane == 0) {
-        if (last) least_s = max(least_s, (uint32_t)(last >> 32) + 1u);
-        queued = found = 0;
-      }
+      const key_t last = sorted[out.k - 1];
+      if (last) least_s = max(least_s, (uint32_t)(last >> 32) + 1u);
+      queued = found = 0;
     }
     __syncthreads();
   }
@@ -227,13 +245,17 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_wait();  // every block of the cluster has started: its shared memory is there
     if (warp == 0) {
-      *cl.map_shared_rank(&lists[rank][lane], 0) = best;
+      if (want_top) *cl.map_shared_rank(&lists[rank][lane], 0) = sorted[lane];
       if (lane == 0) *cl.map_shared_rank(&part_stats[rank], 0) = st;
     }
     cl.sync();
     if (rank != 0) return;
-    if (want_top) best = block_merge_lists(lists, C, warp, lane);
     st = warp_stat(lane < C ? part_stats[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+    if (want_top) {
+      const key_t list = block_merge_lists(lists, C, warp, lane);
+      if (warp == 0) sorted[lane] = list;
+      __syncwarp();
+    }
   } else {
     if (tid == 0) part_stats[0] = st;
     __syncthreads();
@@ -258,6 +280,7 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
       out.logprobs[row * out.G + g] = r;
     }
   if (want_top && warp == 0) {
+    const key_t best = sorted[lane];
     int id = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
     float lp = best ? row_end.logp(order_value((uint32_t)(best >> 32))) : -INFINITY;
     // places left: the first masked elements, then the first NaN
@@ -277,19 +300,19 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
   }
 }
 
-// Blocks a row: 1 to 16, a power of two.  1,024 threads an SM run at a time; a
-// block takes about 5 us to start, to find its alternatives and to join, and
-// one of 256 threads reads 16 KB/us alone or beside another, 11 beside three.
+// Blocks a row: the most, 1 to 16 and a power of two, that leave a block 12 KB
+// while there is a block an SM at most, or 32 KB while there are two.  A cluster
+// costs its blocks about 3 us to join: 148 rows of 131,072 f32 took 35, 24, 30
+// and 34 us with 1, 2, 4 and 8 blocks a row, 37 rows 26, 19, 15 and 15, 301 rows
+// 40, 44, 48 and 62; one row of 50,021 f16 took 13.5, 13.7, 12.0 and 11.2.
 static int pick_cluster(int64_t T, int64_t bytes, int sms) {
-  int best = 1;
-  double least = 0;
-  for (int c = 1; c <= LP_MAX_CLUSTER; c *= 2) {
-    const int64_t blocks = T * c, full = blocks / (4 * sms), rest = blocks % (4 * sms);
-    const double kb = (double)bytes / c / 1000.0;
-    const double cost = full * (5.0 + kb / 11.0) + (rest == 0 ? 0.0 : 5.0 + kb / (rest <= 2 * sms ? 16.0 : 11.0));
-    if (c == 1 || cost < least) best = c, least = cost;
+  int c = 1;
+  while (c < LP_MAX_CLUSTER) {
+    const int64_t blocks = T * 2 * c, share = bytes / (2 * c);
+    if (!(blocks <= sms && share >= 12 * 1024) && !(blocks <= 2 * sms && share >= 32 * 1024)) break;
+    c *= 2;
   }
-  return best;
+  return c;
 }
 
 int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dtype, int64_t T,
@@ -311,8 +334,8 @@ int32_t launch_token_logprobs(har_cuda_ctx *ctx, const void *logits, int32_t dty
       using E = decltype(t);
       // many rows, not the longest: blocks of 128 threads, so that more rows are
       // in different phases and the ends of some overlap the walks of others
-      // (4,096 rows of 5,000 f32: 57 -> 40 us; 2,048 of 131,072 f32: 185 -> 196)
-      const bool narrow = C == 1 && T >= 8 * ctx->num_sms && V * (int64_t)sizeof(E) <= 384 * 1024;
+      // (4,000 rows of 5,000 f32: 63 -> 47 us; 2,400 of 131,072 bf16: 138 -> 144)
+      const bool narrow = C == 1 && T >= 4 * ctx->num_sms && V * (int64_t)sizeof(E) <= 128 * 1024;
       if (C > 8) e = cudaFuncSetAttribute(token_logprobs_kernel<E, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return;
       cudaLaunchConfig_t cfg = {};

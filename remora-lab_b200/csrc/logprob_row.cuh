@@ -36,10 +36,7 @@ __device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
   return {r, a.s + b.s, a.t + b.t};
 }
 __device__ __forceinline__ Stat warp_stat(Stat a) {
-  float r = a.r;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
-  stat_move(a, r);
+  stat_move(a, order_value(__reduce_max_sync(0xffffffffu, order_bits(a.r))));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);

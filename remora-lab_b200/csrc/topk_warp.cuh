@@ -11,12 +11,13 @@ using key_t = unsigned long long;
 template <typename K>
 __device__ __forceinline__ K key_max(K a, K b) { return a > b ? a : b; }
 
-// Descending bitonic sort of one key a lane.
+// Descending bitonic sort of one key a lane.  Rolled: where it runs once, its
+// instructions come from L2.
 template <typename K>
 __device__ __forceinline__ K warp_sort_desc(K v, int lane) {
-#pragma unroll
+#pragma unroll 1
   for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
+#pragma unroll 1
     for (int step = size >> 1; step > 0; step >>= 1) {
       const K o = __shfl_xor_sync(0xffffffffu, v, step);
       const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
@@ -47,6 +48,19 @@ __device__ __forceinline__ key_t warp_take(key_t list, key_t key, uint32_t mask,
     list = lane < pos ? list : lane == pos ? k : up;
   }
   return list;
+}
+
+// The 32 largest of n different keys in shared memory, in descending order (0
+// behind the last): every key counts those above it.  The whole block of
+// `threads`, between barriers; `sorted` was zeroed before the first.
+__device__ __forceinline__ void block_rank(const key_t *keys, int n, key_t *sorted, int tid, int threads) {
+  for (int i = tid; i < n; i += threads) {
+    const key_t mine = keys[i];
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
+    if (above < 32) sorted[above] = mine;
+  }
 }
 
 // n (a power of two, at most twice the block's warps) descending lists at
