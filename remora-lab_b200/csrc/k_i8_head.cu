@@ -143,7 +143,9 @@ __device__ __forceinline__ void list_push(List &l, float v, int32_t id) {
 // Cuts a list back to its k largest entries: the k-th value from a sort of the
 // values alone, then one sweep that keeps what is above it and, of its equals,
 // the first (entries stand in the order of their ids).  The whole warp; a
-// thread with fewer than k entries keeps them and its bar.
+// thread with fewer than k entries keeps them and its bar.  A list holds 32
+// entries and `MORE`.
+template <int MORE>
 __device__ __noinline__ List list_cut(List s, int k) {
   float top[32];
   const int n = s.n();
@@ -153,7 +155,7 @@ __device__ __noinline__ List list_cut(List s, int k) {
   if (__any_sync(0xffffffffu, n > 32)) {
     float more[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) more[i] = 32 + i < n ? list_value(s.at + (32 + i) * H_ROW) : -INFINITY;
+    for (int i = 0; i < 32; ++i) more[i] = i < MORE && 32 + i < n ? list_value(s.at + (32 + i) * H_ROW) : -INFINITY;
     sort32_desc(more);
     merge32_desc(top, more);
   }
@@ -205,9 +207,12 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     float sx = 0.0f;
     int cur = -1;
 
+    auto cut = [&](const List &l) {
+      return p.k > H_LONG ? list_cut<H_CAP_LONG - 32>(l, p.k) : list_cut<H_CAP - 32>(l, p.k);
+    };
     // the token tile's part is done
     auto flush = [&]() {
-      if (p.k > 0) ls = list_cut(ls, p.k);
+      if (p.k > 0) ls = cut(ls);
       if (token >= p.T) return;
       const int64_t part = 2 * tiles.c + h, at = part * p.Tp + token;
       p.part_r[at] = st.r;
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             if (__any_sync(0xffffffffu, top[q] > ls.bar)) {
 #pragma unroll
               for (int i = 8 * q; i < 8 * q + 8; ++i) list_push(ls, l[i], (int32_t)v0 + c + i);
-              if (__any_sync(0xffffffffu, ls.n() > p.full)) ls = list_cut(ls, p.k);
+              if (__any_sync(0xffffffffu, ls.n() > p.full)) ls = cut(ls);
             }
         }
         stat_add<32>(st, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), [&](int i) { return l[i]; });
