@@ -323,7 +323,7 @@ static GemmPlan pick_plan(int64_t M, int64_t N, int64_t K, int sms) {
 
 int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q,
                          int64_t ldq, const float *scale, int64_t M, void *y, int32_t y_dtype,
-                         int64_t ldy) {
+                         int64_t ldy, bool padded) {
   const GemmPlan plan = pick_plan(M, w->N, w->K, ctx->num_sms);
   const int cg = plan.cg;
   GemmParams p = {};
@@ -341,10 +341,10 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
   // store fills the last 16 bytes of a row with zeros)
   TmaDesc map_y = map_x;
   const size_t eb = dtype_bytes(y_dtype);
-  p.store = plan.split == 1 && ((uintptr_t)y & 15u) == 0 && (w->N * (int64_t)eb) % 16 == 0 &&
+  p.store = plan.split == 1 && ((uintptr_t)y & 15u) == 0 && (padded || (w->N * (int64_t)eb) % 16 == 0) &&
             (M == 1 || (ldy * (int64_t)eb) % 16 == 0);
   if (p.store) {
-    const uint64_t pitch = (uint64_t)(M == 1 ? w->N : ldy) * eb;
+    const uint64_t pitch = ((uint64_t)(M == 1 ? w->N : ldy) * eb + 15) / 16 * 16;
     st = encode_tmap_2d(ctx, &map_y, y, (int)eb, (uint64_t)M, (uint64_t)w->N, pitch, 16, G_A, false);
     if (st != HAR_CUDA_OK) return st;
   }

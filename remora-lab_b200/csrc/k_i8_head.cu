@@ -23,7 +23,7 @@ constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
 constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
 constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
-constexpr int64_t H_WALK = 128;     // up to here the logits go through memory
+constexpr int64_t H_WALK_BYTES = 96 << 20, H_WALK_TOKENS = 64;  // up to here the logits go through memory
 
 struct HeadPlan {
   int tt, vt, g, C, passes;         // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
@@ -504,7 +504,16 @@ static int64_t head_chunk(int64_t T) {
   return n == 1 ? T : (c + H_TILE - 1) / H_TILE * H_TILE;
 }
 
-// The logits of a few rows go through memory: scales, q, logits.
+// Whether the logits go through memory: where they stay in L2 a product and a
+// walk take less than the joint kernel, whose blocks bring in a tile of 256
+// tokens beside every tile of weights (203 tokens x 50,021 x 1,999: 68 us
+// against 70 with 3 alternatives and 105 with 20; 256 x 131,072 x 2,048, 134 MB of
+// logits: 117 against 112).
+static bool head_walks(int64_t T, int64_t V) {
+  return T <= H_WALK_TOKENS || T * V <= H_WALK_BYTES / (int64_t)sizeof(float);
+}
+
+// Their places then: scales, q, logits.
 static size_t walk_layout(int64_t T, int64_t V, int64_t K, uint8_t *base, int8_t *&q, float *&sx, float *&logits) {
   sx = (float *)base;
   q = (int8_t *)(base + up(sizeof(float) * (size_t)T));
@@ -517,15 +526,13 @@ size_t head_workspace_bytes(const har_cuda_i8_weights *w, int64_t T, int k) {
   HeadParams p = {};
   int8_t *q;
   float *sx, *logits;
-  if (T <= H_WALK) return walk_layout(T, w->N, w->K, nullptr, q, sx, logits);
+  if (head_walks(T, w->N)) return walk_layout(T, w->N, w->K, nullptr, q, sx, logits);
   const int64_t c = head_chunk(T), rest = T % c;
   const size_t most = head_layout(head_plan(c, w->N, w->sms), c, w->K, k, nullptr, p, q, sx);
   // the last launch is shorter, but its plan may have more parts
   return rest ? std::max(most, head_layout(head_plan(rest, w->N, w->sms), rest, w->K, k, nullptr, p, q, sx)) : most;
 }
 
-// Up to 128 tokens a pair would spend as much of its loads on the token tile
-// as on the weights; the logits stay in L2 instead.
 static int32_t head_walk(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
                          int64_t T, const LogprobOut &out, uint8_t *workspace) {
   int8_t *q;
@@ -537,14 +544,14 @@ static int32_t head_walk(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
     st = launch_i8_gemv(ctx, w, x, x_dtype, ldx, nullptr, T, logits, HAR_CUDA_DTYPE_F32, ldl);
   } else {
     st = launch_i8_quantize(ctx, x, x_dtype, T, w->K, ldx, q, ldq, sx);
-    if (st == HAR_CUDA_OK) st = launch_i8_matmul(ctx, w, q, ldq, sx, T, logits, HAR_CUDA_DTYPE_F32, ldl);
+    if (st == HAR_CUDA_OK) st = launch_i8_matmul(ctx, w, q, ldq, sx, T, logits, HAR_CUDA_DTYPE_F32, ldl, true);
   }
   return st != HAR_CUDA_OK ? st : launch_token_logprobs(ctx, logits, HAR_CUDA_DTYPE_F32, T, w->N, ldl, out);
 }
 
 int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
                        int64_t T, const LogprobOut &out, uint8_t *workspace) {
-  if (T <= H_WALK) return head_walk(ctx, w, x, x_dtype, ldx, T, out, workspace);
+  if (head_walks(T, w->N)) return head_walk(ctx, w, x, x_dtype, ldx, T, out, workspace);
   const int k = out.top_ids || out.top_logprobs ? out.k : 0;
   const int64_t chunk = head_chunk(T), ldq = (w->K + 15) / 16 * 16;
   for (int64_t t0 = 0; t0 < T; t0 += chunk) {

@@ -123,9 +123,11 @@ struct LogprobOut {
 
 int32_t launch_i8_quantize(har_cuda_ctx *ctx, const void *x, int32_t dtype, int64_t M, int64_t K,
                            int64_t ldx, int8_t *q, int64_t ldq, float *scale);
+// padded: y's rows are padded to multiples of 16 bytes, and the padding may be
+// written.
 int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const int8_t *q,
                          int64_t ldq, const float *scale, int64_t M, void *y, int32_t y_dtype,
-                         int64_t ldy);
+                         int64_t ldy, bool padded = false);
 // The product for a few rows: whether it takes these sizes, and the launch, from
 // float rows (sx null: quantised on the way) or from 8-bit rows with scales sx.
 bool i8_gemv_takes(int64_t M, int64_t K);
