@@ -315,8 +315,8 @@ def test_long_rows_and_large_matrices(ctx, dtype, T, V, k):
 @pytest.mark.parametrize("T,V,K,k", [(200, 1, 16, 1), (200, 33, 48, 32), (140, 300, 80, 32), (300, 257, 640, 24),
                                      (1000, 600, 64, 5)])
 def test_head_of_few_rows(ctx, T, V, K, k):
-    """More alternatives than vocabulary, tiles that end early, all above 128
-    tokens."""
+    """More alternatives than vocabulary, tiles that end early, more rows than a
+    tile; the logits stay in the workspace."""
     w, q, s = head_of(ctx, V, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(V)).cuda()
     tok = given(3, T, V, 2)
@@ -325,8 +325,8 @@ def test_head_of_few_rows(ctx, T, V, K, k):
     check_logprobs(got, logprobs64(product(*quantize64(x), q, s, torch.float32), tok, k), (T, V))
 
 
-def test_head_in_several_launches(ctx):
-    """More tokens than one launch takes (4,096): the parts' sizes differ."""
+def test_head_of_many_rows(ctx):
+    """Many rows over a small vocabulary; the logits stay in the workspace."""
     T, V, K, k = 9001, 700, 64, 6
     w, q, s = head_of(ctx, 4, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(5)).cuda()
@@ -356,3 +356,171 @@ def test_head_scales_that_are_not_numbers(ctx, T):
         got = head_score(ctx, wb, x, tok, 32)
         ctx.synchronize()
         check_logprobs(got, logprobs64(product(*quantize64(x), q, s2, torch.float32), tok, 32), (bad, T))
+
+
+# ---- from hidden states, where the logits are not stored ------------------------------
+#
+# More than 64 tokens and more than 25,165,824 logits: the product's epilogue
+# keeps the sums and the lists.  A sample of rows is checked: both ends, the
+# joints between tiles of 128 and 256 tokens, and the special ones.
+
+
+def sample_rows(T):
+    near = [0, 1, 2, 3, 4, 5, 127, 128, 129, 255, 256, 257, 511, 512, T // 2, T - 2, T - 1]
+    return sorted({t for t in near if t < T})
+
+
+def check_large_head(ctx, w, q, s, x, tok, k, rows=None, what=""):
+    T, V = x.shape[0], q.shape[0]
+    assert T > 64 and T * V > 25165824
+    got = head_score(ctx, w, x, tok, k)
+    ctx.synchronize()
+    check_rows(got, q, s, x, tok, k, rows or sample_rows(T), what)
+
+
+def check_rows(got, q, s, x, tok, k, rows, what):
+    logits = product(*quantize64(x[rows]), q, s, torch.float32)
+    check_logprobs({n: v[rows] for n, v in got.items()}, logprobs64(logits, tok[rows], k), what)
+
+
+@pytest.mark.parametrize("T,V,K,G,k,dtype", [(65, 400001, 16, 1, 1, "f32"), (200, 130001, 64, 2, 5, "bf16"),
+                                             (203, 131072, 200, 1, 22, "f32"), (300, 90001, 33, 1, 23, "f16"),
+                                             (257, 100003, 128, 3, 32, "f32"), (1100, 30011, 64, 1, 0, "f32"),
+                                             (4000, 7001, 48, 0, 20, "bf16"), (513, 65537, 1000, 1, 8, "f32")])
+def test_large_head(ctx, T, V, K, G, k, dtype):
+    x = torch.randn(T, K + 3, generator=torch.Generator().manual_seed(T + V)).to(DT[dtype]).cuda()[:, :K]
+    w, q, s = head_of(ctx, V, V, K)
+    tok = given(T, T, V, G)
+    if G:
+        tok[1] = -1
+        tok[0, 0], tok[T - 1, 0] = 0, V - 1
+    check_large_head(ctx, w, q, s, x, tok, k, what=(T, V, K))
+
+
+@pytest.mark.parametrize("k", [5, 22, 32])
+def test_large_head_ties(ctx, k):
+    """Few distinct logits, each many times over: every list is full of equals,
+    and the lower ids stand."""
+    T, V, K = 200, 130001, 16
+    g = torch.Generator().manual_seed(k)
+    q = torch.randint(-1, 2, (V, K), generator=g, dtype=torch.int8).cuda()
+    s = torch.full((V,), 0.25, device="cuda")
+    w = ctx.wrap_i8(q, s)
+    x = torch.randint(-1, 2, (T, K), generator=g).float().cuda()
+    x[3] = 0.0                                  # all equal
+    x[4] = 0.0
+    x[4, 0] = 1.0                               # three values
+    check_large_head(ctx, w, q, s, x, given(k, T, V, 1), k, rows=sample_rows(T)[:8] + [T - 1], what=k)
+
+
+@pytest.mark.parametrize("k", [1, 20, 32])
+def test_large_head_orders(ctx, k):
+    """Logits that rise with the id insert themselves into every list."""
+    T, V, K = 210, 120001, 16
+    q = torch.ones(V, K, dtype=torch.int8, device="cuda")
+    s = torch.linspace(1e-4, 0.02, V).cuda()
+    w = ctx.wrap_i8(q, s)
+    x = torch.ones(T, K, device="cuda")
+    x[1::2] = -1.0                              # and falls
+    check_large_head(ctx, w, q, s, x, given(k, T, V, 1), k, rows=[0, 1, 127, 128, T - 1], what=k)
+
+
+def test_large_head_values_that_are_not_numbers(ctx):
+    """NaN and infinity in x leave the other rows alone; a head scale that is NaN
+    makes every row NaN; scales whose products overflow mask (-inf) what is
+    negative and make a row with a positive one NaN."""
+    T, V, K, k = 200, 130001, 32, 32
+    g = torch.Generator().manual_seed(3)
+    w, q, s = head_of(ctx, 9, V, K)
+    x = torch.randn(T, K, generator=g).cuda()
+    x[2, 5], x[3, 0], x[T - 1] = math.nan, math.inf, 0.0
+    tok = given(4, T, V, 1)
+    check_large_head(ctx, w, q, s, x, tok, k, what="x")
+    s2 = s.clone()
+    s2[V - 100:V - 7] = math.nan
+    check_large_head(ctx, ctx.wrap_i8(q, s2), q, s2, x, tok, k, rows=[0, 2, 128, T - 1], what="nan")
+    # all but ten channels masked in every row, then all of them
+    x = x.nan_to_num(0.5, 0.5, 0.5).abs() + 0.1
+    for live in (10, 0):
+        q2, s2 = -q.abs().clamp(min=1), torch.full((V,), 3e38, device="cuda")
+        if live:
+            at = torch.arange(live, device="cuda") * 12345 + 7
+            s2[at] = 0.01
+        tok[:, 0] = 7
+        tok[5, 0] = 8
+        x2 = 1e3 * x
+        check_large_head(ctx, ctx.wrap_i8(q2, s2), q2, s2, x2, tok, k, rows=[0, 5, 127, 128, T - 1], what=("masked", live))
+    q2[99] = 1                                  # one positive product: +inf
+    check_large_head(ctx, ctx.wrap_i8(q2, s2), q2, s2, x2, tok, k, rows=[0, 128], what="inf")
+
+
+def test_large_head_tokens_outside_the_vocabulary(ctx):
+    T, V, K = 200, 130001, 16
+    w, q, s = head_of(ctx, 10, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(11)).cuda()
+    tok = torch.full((T, 2), -1, dtype=torch.int32, device="cuda")
+    tok[0, 1], tok[T - 1, 0], tok[5] = V, -5, 2
+    got = head_score(ctx, w, x, tok, 4)
+    with pytest.raises(har_cuda.HarCudaError) as e:
+        ctx.synchronize()
+    assert e.value.status == har_cuda.ERR_DEVICE
+    check_rows(got, q, s, x, tok, 4, sample_rows(T), "outside")
+
+
+def test_large_head_captured_and_replayed(ctx):
+    T, V, K, k = 200, 130001, 80, 7
+    w, q, s = head_of(ctx, 12, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(13)).cuda()
+    tok = given(14, T, V, 1)
+    need = w.head_workspace(T, 1, k)
+    work = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    work[need:] = 77
+    o = outputs(T, 1, k)
+    args = (w, x, tok, o["logprobs"], o["entropy"], o["ids"], o["top"])
+    ctx.i8_head_logprobs(*args, workspace=work[:need])
+    torch.cuda.synchronize()
+    first = {n: v.clone() for n, v in o.items()}
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            ctx.bind_torch_stream()
+            ctx.i8_head_logprobs(*args, workspace=work[:need])
+            g.capture_end()
+    finally:
+        ctx.bind_torch_stream()
+    work[:need] = 255
+    g.replay()
+    torch.cuda.synchronize()
+    for n, v in o.items():
+        assert torch.equal(v, first[n]), n      # the same bits from any workspace
+    x.mul_(-1.5)
+    g.replay()
+    torch.cuda.synchronize()
+    check_rows(o, q, s, x, tok, k, sample_rows(T), "replayed")
+    assert bool((work[need:] == 77).all())
+
+
+def test_large_head_in_several_launches(ctx):
+    """9,001 tokens in three launches, the last one shorter."""
+    T, V, K, k = 9001, 3001, 64, 6
+    w, q, s = head_of(ctx, 14, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(5)).cuda()
+    tok = given(6, T, V, 1)
+    rows = list(range(3)) + list(range(3000, 3200)) + list(range(6100, 6200)) + list(range(T - 100, T))
+    check_large_head(ctx, w, q, s, x, tok, k, rows=rows, what="launches")
+
+
+def test_stored_and_unstored_logits_agree(ctx):
+    """The same rows on both paths: 64 of them alone, and among 300."""
+    T, V, K, k = 300, 90001, 96, 20
+    w, q, s = head_of(ctx, 16, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(17)).cuda()
+    tok = given(18, T, V, 1)
+    many, few = head_score(ctx, w, x, tok, k), head_score(ctx, w, x[100:164], tok[100:164], k)
+    ctx.synchronize()
+    assert torch.equal(many["ids"][100:164], few["ids"])
+    # each sum is off by L 2^-22 at the most, L = V / 32 additions, and log by its half steps
+    tol = 2 * (V / 32 * 2.0 ** -22 + 64 * 2.0 ** -24)
+    for n in ("logprobs", "top"):
+        assert float((many[n][100:164] - few[n]).abs().max()) <= tol, n
