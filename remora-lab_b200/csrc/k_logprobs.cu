@@ -138,10 +138,15 @@ __global__ void __launch_bounds__(LP_T, 1024 / LP_T)
     // The k-th largest of 32 of the threads' largest, the best of each warp.
     // (The exact k-th of all, by counting, cost 2,600 cycles.)
     constexpr int EACH = 32 / LP_WARPS;
-    const uint32_t mine = order_bits(most), ranked = warp_sort_desc(mine, lane);
-    if (lane < EACH) tops[EACH * warp + lane] = ranked;
+    const uint32_t mine = order_bits(most);
+    uint32_t rest = mine;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint32_t m = warp_pop_max(rest, lane);
+      if (lane == 0) tops[EACH * warp + i] = m;
+    }
     __syncthreads();
-    const uint32_t bound = max(__shfl_sync(0xffffffffu, warp_sort_desc(tops[lane], lane), out.k - 1), least_s);
+    const uint32_t bound = max(warp_kth(tops[lane], out.k, lane), least_s);
     if (mine >= bound) {
 #pragma unroll 4
       for (int s = 0; s < trips; ++s)

@@ -25,6 +25,21 @@ __device__ __forceinline__ K warp_sort_desc(K v, int lane) {
     }
   return v;
 }
+// The largest of v over the warp, which one lane that has it then gives up.
+__device__ __forceinline__ uint32_t warp_pop_max(uint32_t &v, int lane) {
+  const uint32_t m = __reduce_max_sync(0xffffffffu, v);
+  if (lane == __ffs(__ballot_sync(0xffffffffu, v == m)) - 1) v = 0;
+  return m;
+}
+// The k-th largest (1 to 32) of one value a lane, from the nearer end.
+__device__ __forceinline__ uint32_t warp_kth(uint32_t v, int k, int lane) {
+  const uint32_t flip = k <= 16 ? 0u : ~0u;
+  uint32_t m = 0;
+  v ^= flip;
+#pragma unroll 1
+  for (int i = k <= 16 ? k : 33 - k; i > 0; --i) m = warp_pop_max(v, lane);
+  return m ^ flip;
+}
 // The 32 largest of two descending lists, descending.
 template <typename K>
 __device__ __forceinline__ K warp_merge_desc(K a, K b, int lane) {
