@@ -114,6 +114,16 @@ __device__ __forceinline__ void ring_close(Ring &r, int *status) {
   }
 }
 
+// The ring slot of the next k-step, and the parity of the phase that it is in.
+// Counted along: two divisions a k-step made a loop of one lane's instructions
+// 640 cycles long, more than the MMAs of the largest tile (512).
+struct Slot {
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == (uint32_t)stages) s = 0, phase ^= 1u;
+  }
+};
+
 // One lane loads the A boxes, a lane of another warp the B boxes, of the tiles
 // that `tiles` names: tiles.next(a_row, b_row).
 template <int CG, typename Tiles>
@@ -123,17 +133,18 @@ __device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8
   const int b_rows = sh.bn / CG;
   const uint32_t even = CG == 2 ? tc::cluster_rank() & ~1u : 0u;
   const uint32_t a_bytes = G_A * G_KS, b_bytes = (uint32_t)b_rows * G_KS, bytes = is_b ? b_bytes : a_bytes;
-  uint32_t it = 0;
+  const uint32_t full = CG == 2 ? tc::map_rank(tc::smem_u32(r.full), even) : 0u;
+  uint8_t *const dst = sm + (is_b ? a_bytes : 0);
+  Slot at;
   int a_row, b_row;
   while (tiles.next(a_row, b_row)) {
     const int row = is_b ? b_row + (int)rank * b_rows : a_row + (int)rank * G_A;
-    for (int k = sh.k0; k < sh.k1; ++k, ++it) {
-      const int s = (int)(it % (uint32_t)sh.stages);
-      if (!g_wait(r.empty + s, ((it / (uint32_t)sh.stages) & 1u) ^ 1u, abort_s, 64)) return;
-      uint8_t *dst = sm + (size_t)s * (a_bytes + b_bytes) + (is_b ? a_bytes : 0);
-      if (rank == 0) tc::mbar_expect_tx(r.full + s, CG * bytes);
-      if (CG == 2) tc::tma_load_2d_pair(dst, map, k * G_KS, row, tc::map_rank(tc::smem_u32(r.full + s), even));
-      else tc::tma_load_2d(dst, map, k * G_KS, row, r.full + s);
+    for (int k = sh.k0; k < sh.k1; ++k, at.next(sh.stages)) {
+      if (!tc::mbar_try_wait(r.empty + at.s, at.phase ^ 1u) && !g_wait(r.empty + at.s, at.phase ^ 1u, abort_s, 64)) return;
+      if (rank == 0) tc::mbar_expect_tx(r.full + at.s, CG * bytes);
+      uint8_t *to = dst + at.s * (a_bytes + b_bytes);
+      if (CG == 2) tc::tma_load_2d_pair(to, map, k * G_KS, row, full + at.s * (uint32_t)sizeof(uint64_t));
+      else tc::tma_load_2d(to, map, k * G_KS, row, r.full + at.s);
     }
   }
 }
@@ -144,10 +155,10 @@ __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t
   volatile int *abort_s = &r.abort_flag;
   const int lane = threadIdx.x & 31;
   const uint32_t lead = tc::elect_one(), tmem = r.tmem, even = CG == 2 ? tc::cluster_rank() : 0u;
-  const uint32_t a_bytes = G_A * G_KS, slot = a_bytes + (uint32_t)(sh.bn / CG) * G_KS;
+  const uint32_t a_bytes = G_A * G_KS, slot = a_bytes + (uint32_t)(sh.bn / CG) * G_KS, ring = tc::smem_u32(sm);
   const uint32_t idesc = tc::idesc_i8(CG * G_A, sh.bn);
   const int tail = (int)((sh.K - (int64_t)(sh.k1 - 1) * G_KS + 31) / 32);  // MMAs of the last k-step
-  uint32_t it = 0;
+  Slot at;
   int a_row, b_row;
   for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
     const uint32_t a = n & 1u, par = ((n >> 1) & 1u) ^ 1u;
@@ -164,11 +175,10 @@ __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t
     }
     tc::tc_fence_after();
     const uint32_t d = tmem + a * 256u;
-    for (int k = sh.k0; k < sh.k1; ++k, ++it) {
-      const int s = (int)(it % (uint32_t)sh.stages);
-      if (!g_wait_warp(r.full + s, (it / (uint32_t)sh.stages) & 1u, abort_s, lane)) return;
+    for (int k = sh.k0; k < sh.k1; ++k, at.next(sh.stages)) {
+      if (!g_wait_warp(r.full + at.s, at.phase, abort_s, lane)) return;
       tc::tc_fence_after();
-      const uint32_t base = tc::smem_u32(sm + (size_t)s * slot);
+      const uint32_t base = ring + at.s * slot;
       const uint64_t ad = tc::desc_sw128(base), bd = tc::desc_sw128(base + a_bytes);
       const int slices = k == sh.k1 - 1 ? min(tail, 4) : 4;
 #pragma unroll
@@ -177,8 +187,8 @@ __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t
           if (CG == 2) tc::mma_i8_pair_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, k != sh.k0 || j ? 1u : 0u);
           else tc::mma_i8_ss_w(lead, d, ad + 2 * j, bd + 2 * j, idesc, k != sh.k0 || j ? 1u : 0u);
         }
-      if (CG == 2) tc::mma_commit_pair_w(lead, r.empty + s, even);
-      else tc::mma_commit_w(lead, r.empty + s);
+      if (CG == 2) tc::mma_commit_pair_w(lead, r.empty + at.s, even);
+      else tc::mma_commit_w(lead, r.empty + at.s);
     }
     if (CG == 2) tc::mma_commit_pair_w(lead, r.acc_full + a, even);
     else tc::mma_commit_w(lead, r.acc_full + a);
