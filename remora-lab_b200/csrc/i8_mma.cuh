@@ -54,6 +54,18 @@ __device__ __forceinline__ bool g_wait_warp(uint64_t *bar, uint32_t parity, vola
   return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
 
+// The same for the roles that feed the tensor core: every step of it decided by
+// a vote, so that the loop around it stays uniform and its descriptors,
+// addresses and counters in uniform registers (see elect_one).
+__device__ __forceinline__ bool g_wait_uniform(uint64_t *bar, uint32_t parity, volatile int *abort_s) {
+  for (uint32_t i = 0; i < G_WAIT_LIMIT; ++i) {
+    if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_s)) return false;
+  }
+  *abort_s = 1;
+  return false;
+}
+
 template <int CG>
 __device__ __forceinline__ void ring_open(Ring &r, const RingShape &sh, const void *map_a, const void *map_b) {
   const int tid = threadIdx.x;
@@ -124,27 +136,27 @@ struct Slot {
   }
 };
 
-// One lane loads the A boxes, a lane of another warp the B boxes, of the tiles
-// that `tiles` names: tiles.next(a_row, b_row).
+// One warp loads the A boxes, another the B boxes, of the tiles that `tiles`
+// names: tiles.next(a_row, b_row).
 template <int CG, typename Tiles>
 __device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8_t *sm, bool is_b, const void *map,
                                              Tiles tiles, uint32_t rank) {
   volatile int *abort_s = &r.abort_flag;
   const int b_rows = sh.bn / CG;
-  const uint32_t even = CG == 2 ? tc::cluster_rank() & ~1u : 0u;
+  const uint32_t lead = tc::elect_one(), even = CG == 2 ? tc::cluster_rank() & ~1u : 0u;
   const uint32_t a_bytes = G_A * G_KS, b_bytes = (uint32_t)b_rows * G_KS, bytes = is_b ? b_bytes : a_bytes;
-  const uint32_t full = CG == 2 ? tc::map_rank(tc::smem_u32(r.full), even) : 0u;
-  uint8_t *const dst = sm + (is_b ? a_bytes : 0);
+  const uint32_t full = tc::smem_u32(r.full), full_even = CG == 2 ? tc::map_rank(full, even) : full;
+  const uint32_t dst = tc::smem_u32(sm) + (is_b ? a_bytes : 0u);
   Slot at;
   int a_row, b_row;
   while (tiles.next(a_row, b_row)) {
     const int row = is_b ? b_row + (int)rank * b_rows : a_row + (int)rank * G_A;
     for (int k = sh.k0; k < sh.k1; ++k, at.next(sh.stages)) {
-      if (!tc::mbar_try_wait(r.empty + at.s, at.phase ^ 1u) && !g_wait(r.empty + at.s, at.phase ^ 1u, abort_s, 64)) return;
-      if (rank == 0) tc::mbar_expect_tx(r.full + at.s, CG * bytes);
-      uint8_t *to = dst + at.s * (a_bytes + b_bytes);
-      if (CG == 2) tc::tma_load_2d_pair(to, map, k * G_KS, row, full + at.s * (uint32_t)sizeof(uint64_t));
-      else tc::tma_load_2d(to, map, k * G_KS, row, r.full + at.s);
+      if (!g_wait_uniform(r.empty + at.s, at.phase ^ 1u, abort_s)) return;
+      const uint32_t to = dst + at.s * (a_bytes + b_bytes), bar = at.s * (uint32_t)sizeof(uint64_t);
+      if (rank == 0) tc::mbar_expect_tx_w(lead, full + bar, CG * bytes);
+      if (CG == 2) tc::tma_load_2d_pair_w(lead, to, map, k * G_KS, row, full_even + bar);
+      else tc::tma_load_2d_w(lead, to, map, k * G_KS, row, full + bar);
     }
   }
 }
@@ -153,8 +165,8 @@ __device__ __forceinline__ void ring_produce(Ring &r, const RingShape &sh, uint8
 template <int CG, typename Tiles>
 __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t *sm, Tiles tiles) {
   volatile int *abort_s = &r.abort_flag;
-  const int lane = threadIdx.x & 31;
-  const uint32_t lead = tc::elect_one(), tmem = r.tmem, even = CG == 2 ? tc::cluster_rank() : 0u;
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, r.tmem);  // one value, in a uniform register
+  const uint32_t lead = tc::elect_one(), even = CG == 2 ? tc::cluster_rank() : 0u;
   const uint32_t a_bytes = G_A * G_KS, slot = a_bytes + (uint32_t)(sh.bn / CG) * G_KS, ring = tc::smem_u32(sm);
   const uint32_t idesc = tc::idesc_i8(CG * G_A, sh.bn);
   const int tail = (int)((sh.K - (int64_t)(sh.k1 - 1) * G_KS + 31) / 32);  // MMAs of the last k-step
@@ -163,20 +175,20 @@ __device__ __forceinline__ void ring_issue(Ring &r, const RingShape &sh, uint8_t
   for (uint32_t n = 0; tiles.next(a_row, b_row); ++n) {
     const uint32_t a = n & 1u, par = ((n >> 1) & 1u) ^ 1u;
     if (CG == 2) {  // arrivals of both blocks
-      bool ok = true;
-      if (lane == 0) {
-        ok = false;
-        for (uint32_t i = 0; i < G_WAIT_LIMIT && !ok && !*abort_s; ++i) ok = tc::mbar_try_wait_cluster(r.acc_empty + a, par);
-        if (!ok) *abort_s = 1;
+      bool ok = false;
+      for (uint32_t i = 0; i < G_WAIT_LIMIT && !ok && !__any_sync(0xffffffffu, *abort_s); ++i)
+        ok = __all_sync(0xffffffffu, tc::mbar_try_wait_cluster(r.acc_empty + a, par));
+      if (!ok) {
+        *abort_s = 1;
+        return;
       }
-      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) return;
-    } else if (!g_wait_warp(r.acc_empty + a, par, abort_s, lane)) {
+    } else if (!g_wait_uniform(r.acc_empty + a, par, abort_s)) {
       return;
     }
     tc::tc_fence_after();
     const uint32_t d = tmem + a * 256u;
     for (int k = sh.k0; k < sh.k1; ++k, at.next(sh.stages)) {
-      if (!g_wait_warp(r.full + at.s, at.phase, abort_s, lane)) return;
+      if (!g_wait_uniform(r.full + at.s, at.phase, abort_s)) return;
       tc::tc_fence_after();
       const uint32_t base = ring + at.s * slot;
       const uint64_t ad = tc::desc_sw128(base), bd = tc::desc_sw128(base + a_bytes);

@@ -139,9 +139,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   ring_open<CG>(ring, p.sh, &map_w, &map_x);
 
   if (warp == G_WARP_A) {
-    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, false, &map_w, GemmTiles<CG>(p), rank);
+    ring_produce<CG>(ring, p.sh, sm, false, &map_w, GemmTiles<CG>(p), rank);
   } else if (warp == G_WARP_B) {
-    if (lane == 0) ring_produce<CG>(ring, p.sh, sm, true, &map_x, GemmTiles<CG>(p), rank);
+    ring_produce<CG>(ring, p.sh, sm, true, &map_x, GemmTiles<CG>(p), rank);
   } else if (warp == G_WARP_MMA) {
     if (rank == 0) ring_issue<CG>(ring, p.sh, sm, GemmTiles<CG>(p));
   } else {
@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   uint32_t v[4][32];
   bool ok = false;
   if (warp == G_WARP_A) {
-    if (lane == 0) ring_produce<2>(ring, p.sh, sm, false, &map_w, one, rank);
+    ring_produce<2>(ring, p.sh, sm, false, &map_w, one, rank);
   } else if (warp == G_WARP_B) {
-    if (lane == 0) ring_produce<2>(ring, p.sh, sm, true, &map_x, one, rank);
+    ring_produce<2>(ring, p.sh, sm, true, &map_x, one, rank);
   } else if (warp == G_WARP_MMA) {
     if (rank == 0) ring_issue<2>(ring, p.sh, sm, one);
   } else {

@@ -188,9 +188,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   ring_open<2>(ring, p.sh, &map_x, &map_w);
 
   if (warp == G_WARP_A) {
-    if (lane == 0) ring_produce<2>(ring, p.sh, sm, false, &map_x, HeadTiles(p), rank);
+    ring_produce<2>(ring, p.sh, sm, false, &map_x, HeadTiles(p), rank);
   } else if (warp == G_WARP_B) {
-    if (lane == 0) ring_produce<2>(ring, p.sh, sm, true, &map_w, HeadTiles(p), rank);
+    ring_produce<2>(ring, p.sh, sm, true, &map_w, HeadTiles(p), rank);
   } else if (warp == G_WARP_MMA) {
     if (rank == 0) ring_issue<2>(ring, p.sh, sm, HeadTiles(p));
   } else {

@@ -292,6 +292,34 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *tmap, in
       "l"(tmap), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// The same loads, and the arrival that announces their bytes, by the lane of a
+// whole warp whose `lead` is not 0: see elect_one.
+__device__ __forceinline__ void tma_load_2d_w(uint32_t lead, uint32_t dst, const void *tmap, int x, int y, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(tmap), "r"(x), "r"(y), "r"(bar), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair_w(uint32_t lead, uint32_t dst, const void *tmap, int x, int y, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(tmap), "r"(x), "r"(y), "r"(bar), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_w(uint32_t lead, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %2, 0;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(lead)
+      : "memory");
+}
 // Both CTAs' warps call these together.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
