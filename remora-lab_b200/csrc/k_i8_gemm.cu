@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 }
 
 // The same product where there are fewer tiles than pairs: a cluster of S pairs
-// shares one tile, each pair a part of K, because a block alone brings in no
-// more than about 65 GB/s (512 x 2048 x 2048: 16 k-steps took 5.1 us whatever
-// the tile's size).  The pairs leave their 32-bit sums in their shared memory;
+// shares one tile, each pair a part of K, because a k-step takes its 315 cycles
+// however narrow the tile (8 x 512 x 16,384: 24.6 us whole, 15.4 in four parts;
+// 8 x 2,048 x 8,192: 16.2 and 10.8).  The pairs leave their 32-bit sums in their shared memory;
 // pair s reads every pair's sums of token slice s, adds them up (whole numbers:
 // any order) and writes its slice.  (Sent instead of fetched they took two
 // barriers and 3.3 us for the smallest tile.)
@@ -290,13 +290,16 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 }
 
 // How a product is cut up.  Blocks a tile (cg), tokens of a tile (bn), pairs
-// that share a tile (split): the cheapest by these measures.  A k-step of a
-// tile costs a lone block its MMAs (2 cycles a token at 8,192 products a cycle)
-// or its bytes from L2 (about 42 a cycle measured, with all blocks loading) or
-// 540 cycles, the time a box of 128 rows takes at the least; a pair moves half
-// the token bytes.  A tile costs about 1,500 cycles to fill and drain, a pair
-// 500 more to join, and 2,500 if its sums have to meet.  Clusters of 4 and 8
-// blocks do not fill every group of SMs: 35 and 15 of them ran at a time.
+// that share a tile (split): the cheapest by these measures.  A k-step costs a
+// block its MMAs, 2 cycles a token at 8,192 products a cycle, and 315 at the
+// least, which issuing them takes; or its bytes, 72 a cycle, of which a pair's
+// blocks share the tokens'.  A tile costs about 1,000 cycles to fill and drain,
+// a pair 2,000 more to join, and 4,000 if its sums have to meet.  Of 220 cuts of
+// 31 products from 64 x 64 x 64 to 4096^3 the cut that it names is 1.5% slower
+// than the best on average: 777 x 5,008 x 1,999 takes 19.6 us as 280 lone tiles of
+// 112 tokens and 19.9 as 140 pairs' of 128, 203 x 50,024 x 1,999 44 us alone and 38
+// in pairs, 4096^3 54 and 51.  Clusters of 4 and 8 blocks do not fill every
+// group of SMs: 35 and 15 of them ran at a time.
 struct GemmPlan {
   int cg, bn, split;
 };
@@ -309,11 +312,11 @@ static GemmPlan pick_plan(int64_t M, int64_t N, int64_t K, int sms) {
     for (int64_t mt = first; mt <= first + 15; ++mt) {
       const int64_t b = ((M + mt - 1) / mt + 16 * g - 1) / (16 * g) * (16 * g);
       const int64_t tiles = nt * ((M + b - 1) / b);
-      const double step = std::max({2.0 * b, (G_A * G_KS + b / g * G_KS) / 42.0, 540.0});
+      const double step = std::max({2.0 * b, (G_A + b / g) * (G_KS / 72.0), 315.0});
       for (int s = 1; s <= (g == 2 ? 4 : 1); s *= 2) {
         if (s > 1 && (tiles > (s == 2 ? 35 : 15) * sms / 148 || ksteps < 2 * s)) continue;
         const int64_t waves = (tiles * s + sms / g - 1) / (sms / g);
-        const double cost = waves * ((ksteps + s - 1) / s * step + 1500.0 + 500.0 * (g - 1)) + (s > 1 ? 2500.0 : 0.0);
+        const double cost = waves * ((ksteps + s - 1) / s * step + 1000.0 + 2000.0 * (g - 1)) + (s > 1 ? 4000.0 : 0.0);
         if (!plan.bn || cost < best) best = cost, plan = {g, (int)b, s};
       }
     }
