@@ -23,7 +23,7 @@ constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
 constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
 constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
-constexpr int64_t H_WALK_BYTES = 96 << 20, H_WALK_TOKENS = 64;  // up to here the logits go through memory
+constexpr int64_t H_WALK_TOKENS = 64, H_WALK_BYTES = 16 << 20;
 
 struct HeadPlan {
   int tt, vt, g, C, passes;         // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
@@ -504,13 +504,17 @@ static int64_t head_chunk(int64_t T) {
   return n == 1 ? T : (c + H_TILE - 1) / H_TILE * H_TILE;
 }
 
-// Whether the logits go through memory: where they stay in L2 a product and a
-// walk take less than the joint kernel, whose blocks bring in a tile of 256
-// tokens beside every tile of weights (203 tokens x 50,021 x 1,999: 68 us
-// against 70 with 3 alternatives and 105 with 20; 256 x 131,072 x 2,048, 134 MB of
-// logits: 117 against 112).
-static bool head_walks(int64_t T, int64_t V) {
-  return T <= H_WALK_TOKENS || T * V <= H_WALK_BYTES / (int64_t)sizeof(float);
+// Whether the logits go through memory.  A product and a walk do for up to 64
+// tokens, of which a tile of 256 makes little (64 x 131,072 x 4,096: 110 us against
+// 118), and where the lists that every part of a row keeps cost more than the
+// logits' way: that grows with the alternatives.  For 256 x 131,072 x 2,048 the
+// walk takes 110 to 115 us, this kernel 72, 89, 95, 105, 114, 121 and 149 with 0, 1,
+// 2, 5, 8, 12 and 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 63, 67, 72
+// (5) and 103 (20); for 2,048 x 32,000 x 2,048 170 (8), 176 (20) and 187 (32),
+// and 164, 229 and 300; for 768 x 131,072 x 2,048 252 (8), 254 and 262, and 218,
+// 293 and 378.
+static bool head_walks(int64_t T, int64_t V, int k) {
+  return T <= H_WALK_TOKENS || T * V * (int64_t)sizeof(float) <= (k ? std::max(k, 8) : 1) * H_WALK_BYTES;
 }
 
 // Their places then: scales, q, logits.
@@ -526,7 +530,7 @@ size_t head_workspace_bytes(const har_cuda_i8_weights *w, int64_t T, int k) {
   HeadParams p = {};
   int8_t *q;
   float *sx, *logits;
-  if (head_walks(T, w->N)) return walk_layout(T, w->N, w->K, nullptr, q, sx, logits);
+  if (head_walks(T, w->N, k)) return walk_layout(T, w->N, w->K, nullptr, q, sx, logits);
   const int64_t c = head_chunk(T), rest = T % c;
   const size_t most = head_layout(head_plan(c, w->N, w->sms), c, w->K, k, nullptr, p, q, sx);
   // the last launch is shorter, but its plan may have more parts
@@ -551,7 +555,7 @@ static int32_t head_walk(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
 
 int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype, int64_t ldx,
                        int64_t T, const LogprobOut &out, uint8_t *workspace) {
-  if (head_walks(T, w->N)) return head_walk(ctx, w, x, x_dtype, ldx, T, out, workspace);
+  if (head_walks(T, w->N, out.k)) return head_walk(ctx, w, x, x_dtype, ldx, T, out, workspace);
   const int k = out.top_ids || out.top_logprobs ? out.k : 0;
   const int64_t chunk = head_chunk(T), ldq = (w->K + 15) / 16 * 16;
   for (int64_t t0 = 0; t0 < T; t0 += chunk) {

@@ -360,9 +360,13 @@ def test_head_scales_that_are_not_numbers(ctx, T):
 
 # ---- from hidden states, where the logits are not stored ------------------------------
 #
-# More than 64 tokens and more than 25,165,824 logits: the product's epilogue
-# keeps the sums and the lists.  A sample of rows is checked: both ends, the
-# joints between tiles of 128 and 256 tokens, and the special ones.
+# More than 64 tokens and more than 16 MB of logits, times the alternatives: the
+# product's epilogue keeps the sums and the lists.  A sample of rows is checked:
+# both ends, the joints between tiles of 128 and 256 tokens, and the special ones.
+
+
+def unstored(T, V, k):
+    return T > 64 and 4 * T * V > (max(k, 8) if k else 1) * 2 ** 24
 
 
 def sample_rows(T):
@@ -372,7 +376,7 @@ def sample_rows(T):
 
 def check_large_head(ctx, w, q, s, x, tok, k, rows=None, what=""):
     T, V = x.shape[0], q.shape[0]
-    assert T > 64 and T * V > 25165824
+    assert unstored(T, V, k)
     got = head_score(ctx, w, x, tok, k)
     ctx.synchronize()
     check_rows(got, q, s, x, tok, k, rows or sample_rows(T), what)
@@ -383,10 +387,11 @@ def check_rows(got, q, s, x, tok, k, rows, what):
     check_logprobs({n: v[rows] for n, v in got.items()}, logprobs64(logits, tok[rows], k), what)
 
 
-@pytest.mark.parametrize("T,V,K,G,k,dtype", [(65, 400001, 16, 1, 1, "f32"), (200, 130001, 64, 2, 5, "bf16"),
-                                             (203, 131072, 200, 1, 22, "f32"), (300, 90001, 33, 1, 23, "f16"),
-                                             (257, 100003, 128, 3, 32, "f32"), (1100, 30011, 64, 1, 0, "f32"),
-                                             (4000, 7001, 48, 0, 20, "bf16"), (513, 65537, 1000, 1, 8, "f32")])
+@pytest.mark.parametrize("T,V,K,G,k,dtype", [(65, 600001, 16, 1, 1, "f32"), (200, 200001, 64, 2, 5, "bf16"),
+                                             (203, 460001, 72, 1, 22, "f32"), (300, 330001, 33, 1, 23, "f16"),
+                                             (257, 530003, 40, 3, 32, "f32"), (1100, 30011, 64, 1, 0, "f32"),
+                                             (4000, 21001, 48, 0, 20, "bf16"), (513, 65537, 1000, 1, 8, "f32"),
+                                             (130, 40000, 100, 1, 0, "f16")])
 def test_large_head(ctx, T, V, K, G, k, dtype):
     x = torch.randn(T, K + 3, generator=torch.Generator().manual_seed(T + V)).to(DT[dtype]).cuda()[:, :K]
     w, q, s = head_of(ctx, V, V, K)
@@ -401,7 +406,7 @@ def test_large_head(ctx, T, V, K, G, k, dtype):
 def test_large_head_ties(ctx, k):
     """Few distinct logits, each many times over: every list is full of equals,
     and the lower ids stand."""
-    T, V, K = 200, 130001, 16
+    T, V, K = 200, 700001, 16
     g = torch.Generator().manual_seed(k)
     q = torch.randint(-1, 2, (V, K), generator=g, dtype=torch.int8).cuda()
     s = torch.full((V,), 0.25, device="cuda")
@@ -416,7 +421,7 @@ def test_large_head_ties(ctx, k):
 @pytest.mark.parametrize("k", [1, 20, 32])
 def test_large_head_orders(ctx, k):
     """Logits that rise with the id insert themselves into every list."""
-    T, V, K = 210, 120001, 16
+    T, V, K = 210, 640001, 16
     q = torch.ones(V, K, dtype=torch.int8, device="cuda")
     s = torch.linspace(1e-4, 0.02, V).cuda()
     w = ctx.wrap_i8(q, s)
@@ -429,7 +434,7 @@ def test_large_head_values_that_are_not_numbers(ctx):
     """NaN and infinity in x leave the other rows alone; a head scale that is NaN
     makes every row NaN; scales whose products overflow mask (-inf) what is
     negative and make a row with a positive one NaN."""
-    T, V, K, k = 200, 130001, 32, 32
+    T, V, K, k = 200, 680001, 32, 32
     g = torch.Generator().manual_seed(3)
     w, q, s = head_of(ctx, 9, V, K)
     x = torch.randn(T, K, generator=g).cuda()
@@ -455,7 +460,8 @@ def test_large_head_values_that_are_not_numbers(ctx):
 
 
 def test_large_head_tokens_outside_the_vocabulary(ctx):
-    T, V, K = 200, 130001, 16
+    T, V, K = 200, 200001, 16
+    assert unstored(T, V, 4)
     w, q, s = head_of(ctx, 10, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(11)).cuda()
     tok = torch.full((T, 2), -1, dtype=torch.int32, device="cuda")
@@ -468,7 +474,8 @@ def test_large_head_tokens_outside_the_vocabulary(ctx):
 
 
 def test_large_head_captured_and_replayed(ctx):
-    T, V, K, k = 200, 130001, 80, 7
+    T, V, K, k = 200, 200001, 80, 7
+    assert unstored(T, V, k)
     w, q, s = head_of(ctx, 12, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(13)).cuda()
     tok = given(14, T, V, 1)
@@ -503,7 +510,7 @@ def test_large_head_captured_and_replayed(ctx):
 
 def test_large_head_in_several_launches(ctx):
     """9,001 tokens in three launches, the last one shorter."""
-    T, V, K, k = 9001, 3001, 64, 6
+    T, V, K, k = 9001, 4001, 64, 6
     w, q, s = head_of(ctx, 14, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(5)).cuda()
     tok = given(6, T, V, 1)
@@ -513,7 +520,8 @@ def test_large_head_in_several_launches(ctx):
 
 def test_stored_and_unstored_logits_agree(ctx):
     """The same rows on both paths: 64 of them alone, and among 300."""
-    T, V, K, k = 300, 90001, 96, 20
+    T, V, K, k = 300, 290001, 96, 20
+    assert unstored(T, V, k)
     w, q, s = head_of(ctx, 16, V, K)
     x = torch.randn(T, K, generator=torch.Generator().manual_seed(17)).cuda()
     tok = given(18, T, V, 1)
