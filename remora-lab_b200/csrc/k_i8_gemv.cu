@@ -174,12 +174,15 @@ __global__ void __launch_bounds__(V_T, 2) i8_gemv_kernel(const GemvParams p) {
   }
 }
 
-// Up to 4 rows: above, the tensor cores' launch and its quantising pass cost
-// less than quantising the rows in every block and 8 dp4a a byte (5 to 8 rows
-// of 131072 x 4096 measured 149 us here, 95 us there; 4 rows 98 and 95).
-bool i8_gemv_takes(int64_t M, int64_t K) {
-  const int64_t mt = M <= 1 ? 1 : M <= 2 ? 2 : 4;
-  return M <= 4 && mt * ((K + 15) / 16 * 16) <= V_MAX_SMEM;
+static int gemv_rows(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
+
+// Up to 4 rows, and 8 of a small matrix: above, the tensor cores' launch and its
+// quantising pass cost less than quantising the rows in every block and a dp4a
+// a row and four bytes (131,072 x 4,096: 80 us here and 91 there for 2 rows, 96 and
+// 91 for 4; 4,096 x 2,048: 8.3 and 13.7 for 4 rows, 10.6 and 12.9 for 8;
+// 4,096 x 4,096: 16.6 and 15.0 for 8).
+bool i8_gemv_takes(int64_t M, int64_t N, int64_t K) {
+  return (M <= 4 || (M <= 8 && N * K <= 8 << 20)) && gemv_rows(M) * ((K + 15) / 16 * 16) <= V_MAX_SMEM;
 }
 
 int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype,
@@ -189,7 +192,7 @@ int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
   p.x = x, p.sx = sx, p.ldx = ldx, p.x_dtype = x_dtype, p.M = (int)M, p.y = y, p.ldy = ldy;
   const size_t eb = dtype_bytes(x_dtype);
   p.wide = sx == nullptr && ((uintptr_t)x & (4 * eb - 1)) == 0 && (M == 1 || ldx % 4 == 0);
-  const int mt = M <= 1 ? 1 : M <= 2 ? 2 : 4;
+  const int mt = gemv_rows(M);
   const size_t smem = (size_t)mt * (size_t)((w->K + 15) / 16 * 16);
   const int64_t blocks = (w->N + V_WARPS * V_R - 1) / (V_WARPS * V_R);
   const unsigned grid = (unsigned)std::min<int64_t>(blocks, 2 * ctx->num_sms);
@@ -203,7 +206,8 @@ int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     using T = decltype(t);
     if (mt == 1) go(i8_gemv_kernel<T, 1>);
     else if (mt == 2) go(i8_gemv_kernel<T, 2>);
-    else go(i8_gemv_kernel<T, 4>);
+    else if (mt == 4) go(i8_gemv_kernel<T, 4>);
+    else go(i8_gemv_kernel<T, 8>);
   });
   const int32_t st = check_launch(ctx, "i8_gemv_kernel");
   if (e != cudaSuccess)

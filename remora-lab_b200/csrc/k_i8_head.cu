@@ -544,7 +544,7 @@ static int32_t head_walk(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
   walk_layout(T, w->N, w->K, workspace, q, sx, logits);
   const int64_t ldq = (w->K + 15) / 16 * 16, ldl = (w->N + 3) / 4 * 4;
   int32_t st;
-  if (i8_gemv_takes(T, w->K)) {
+  if (i8_gemv_takes(T, w->N, w->K)) {
     st = launch_i8_gemv(ctx, w, x, x_dtype, ldx, nullptr, T, logits, HAR_CUDA_DTYPE_F32, ldl);
   } else {
     st = launch_i8_quantize(ctx, x, x_dtype, T, w->K, ldx, q, ldq, sx);

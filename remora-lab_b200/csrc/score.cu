@@ -209,7 +209,7 @@ int32_t har_cuda_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
   OnDevice on(ctx);
   HAR_TRY(on.status(ctx));
   if (M == 1) ldq = (int64_t)round16((size_t)w->K), ldy = w->N;
-  if (i8_gemv_takes(M, w->K)) return launch_i8_gemv(ctx, w, q_dev, 0, ldq, scale_dev, M, y_dev, y_dtype, ldy);
+  if (i8_gemv_takes(M, w->N, w->K)) return launch_i8_gemv(ctx, w, q_dev, 0, ldq, scale_dev, M, y_dev, y_dtype, ldy);
   return launch_i8_matmul(ctx, w, q_dev, ldq, scale_dev, M, y_dev, y_dtype, ldy);
 }
 
@@ -220,7 +220,7 @@ static size_t quantized_bytes(const har_cuda_i8_weights *w, int64_t M) {
 
 int64_t har_cuda_i8_linear_workspace(const har_cuda_i8_weights *w, int64_t M) {
   if (!w || M < 0 || M > I8_MAX_ROWS) return -1;
-  return M == 0 || i8_gemv_takes(M, w->K) ? 0 : (int64_t)quantized_bytes(w, M);
+  return M == 0 || i8_gemv_takes(M, w->N, w->K) ? 0 : (int64_t)quantized_bytes(w, M);
 }
 
 int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x_dev,
@@ -237,7 +237,7 @@ int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
   OnDevice on(ctx);
   HAR_TRY(on.status(ctx));
   if (M == 1) ldx = w->K, ldy = w->N;
-  if (i8_gemv_takes(M, w->K)) return launch_i8_gemv(ctx, w, x_dev, x_dtype, ldx, nullptr, M, y_dev, y_dtype, ldy);
+  if (i8_gemv_takes(M, w->N, w->K)) return launch_i8_gemv(ctx, w, x_dev, x_dtype, ldx, nullptr, M, y_dev, y_dtype, ldy);
   uint8_t *ws;
   HAR_TRY(take_workspace(ctx, workspace_dev, workspace_bytes, quantized_bytes(w, M), "i8_linear", &ws));
   float *scale = (float *)ws;

@@ -130,7 +130,7 @@ int32_t launch_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const 
                          int64_t ldy, bool padded = false);
 // The product for a few rows: whether it takes these sizes, and the launch, from
 // float rows (sx null: quantised on the way) or from 8-bit rows with scales sx.
-bool i8_gemv_takes(int64_t M, int64_t K);
+bool i8_gemv_takes(int64_t M, int64_t N, int64_t K);
 int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x, int32_t x_dtype,
                        int64_t ldx, const float *sx, int64_t M, void *y, int32_t y_dtype, int64_t ldy);
 // The whole head call on a workspace of head_workspace_bytes.

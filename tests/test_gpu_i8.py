@@ -113,7 +113,9 @@ SHAPES = [(1, 1, 1), (1, 3, 16), (1, 130, 2048), (2, 64, 15), (3, 127, 17), (4, 
           (8, 257, 128), (9, 33, 144), (15, 128, 256), (16, 300, 63), (17, 255, 129), (31, 1000, 512),
           (33, 513, 1040), (64, 128, 2048), (65, 140, 300), (128, 384, 1000), (129, 640, 96), (256, 129, 272),
           (257, 256, 4096), (300, 1031, 777), (513, 260, 1024), (700, 5, 33), (1025, 515, 160), (2050, 1300, 720), (513, 5003, 96), (4100, 300, 48), (16, 1000, 2048),
-          (100, 700, 1153), (512, 1500, 1100), (40, 3000, 600)]
+          (100, 700, 1153), (512, 1500, 1100), (40, 3000, 600),
+          # 5 to 8 rows: of a small matrix, of one just too large, with the longest rows on either side
+          (5, 1, 1), (6, 1000, 2051), (8, 4096, 2048), (8, 8200, 1100), (5, 3, 12285), (8, 70, 12300)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -161,7 +163,7 @@ def test_extreme_sums(ctx, M):
     assert torch.equal(y.cpu(), product(rq, rs, wq, ws, torch.float32))
 
 
-@pytest.mark.parametrize("M", [2, 20, 200])
+@pytest.mark.parametrize("M", [2, 6, 20, 200])
 def test_rows_that_are_not_numbers(ctx, M):
     x = rows(5, M, 100)
     x[1, 3] = math.nan
