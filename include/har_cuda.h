@@ -164,6 +164,9 @@ int32_t har_cuda_q3k_gemv(har_cuda_ctx *ctx, const har_cuda_weights *w, int64_t 
 /* ---- 8-bit integer products with scales per token and channel ----------------
  * No reference counterpart: the dense product of many token rows (an LM head
  * over a prompt, a projection) that the block-quantised GEMVs above leave out.
+ * In this section and the next, outputs and workspaces overlap neither each
+ * other nor any input; results do not depend on the workspace or on what ran
+ * before, and are the same bits from call to call.
  * Element types of float operands: */
 #define HAR_CUDA_DTYPE_F32 0
 #define HAR_CUDA_DTYPE_F16 1
@@ -233,9 +236,11 @@ int32_t har_cuda_token_logprobs(har_cuda_ctx *ctx, const void *logits_dev, int32
                                 int32_t k, float *logprobs_dev, float *entropy_dev,
                                 int32_t *top_ids_dev, float *top_logprobs_dev);
 /* har_cuda_token_logprobs of the logits that har_cuda_i8_linear would write as
- * f32 for the LM head w [V][K] and hidden states x_dev [T][K], without the
- * [T][V] logits in memory.  Workspace as for har_cuda_i8_linear, of
- * har_cuda_i8_head_workspace bytes. */
+ * f32 for the LM head w [V][K] and hidden states x_dev [T][K].  The logits of
+ * many rows never reach memory; those of up to 64 rows, and up to 16 MB of them
+ * (times max(k, 8) with alternatives), pass through the workspace, where that is
+ * faster.  Workspace as for har_cuda_i8_linear, of har_cuda_i8_head_workspace
+ * bytes for this T and k (one for k serves k = 0 too). */
 int64_t har_cuda_i8_head_workspace(const har_cuda_i8_weights *w, int64_t T, int32_t G, int32_t k);
 int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *w,
                                   const void *x_dev, int32_t x_dtype, int64_t ldx, int64_t T,

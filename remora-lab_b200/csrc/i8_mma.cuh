@@ -5,11 +5,12 @@
 //
 // CG = 1: a block computes tiles of 128 A rows x bn B rows.  CG = 2: a cluster
 // of two computes tiles of 256 x bn; each block loads its own 128 rows of A and
-// half the rows of B, so a k-step of 128 bytes brings 32 KB into a block's
-// shared memory for the same products that cost a lone block 48 KB.  Shared
-// memory moves 128 bytes a cycle and every byte crosses it twice (in by TMA,
-// out to the tensor core): a lone block at bn = 256 needs 750 cycles for 512
-// cycles of MMAs, a pair 512 for 512.
+// half the rows of B, so at bn = 256 a k-step of 128 bytes brings 32 KB into a
+// block's shared memory for the products that cost a lone block 48 KB.  Either
+// takes max(2 bn, 315) cycles once the bytes are there; with 148 blocks loading
+// from memory and L2 (256 x 18,944 x 8,192) it took 983 cycles alone and 838 in
+// pairs.  A lone tile's advantage is its size: half the channels, so fewer
+// blocks stand idle in the last round of a product of few tiles.
 #pragma once
 
 #include "score.cuh"

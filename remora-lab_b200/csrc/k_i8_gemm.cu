@@ -1,5 +1,7 @@
 // k_i8_gemm.cu — y = (q_x q_w^T) * s_x * s_w over 8-bit integers on the tensor
 // cores (tcgen05.mma kind::i8, 32-bit sums in tensor memory).
+// 8,192 x 8,192 x 4,096 in bf16: 172 us, 3.2 POP/s, the tensor pipe active for 92% of
+// the cycles; 48 x 65,536 x 2,048 in f32: 29 us, 5.1 TB/s of weights and output.
 #include <algorithm>
 
 #include "i8_mma.cuh"
@@ -83,9 +85,11 @@ __device__ __forceinline__ void put_rows(T *y, int64_t ldy, const T *slab, int t
 // Output of `n` tokens (at most 128, from token m) of 128 channels, by the
 // four warps of one half; v holds this thread's channel.  Finished values are
 // laid out in shared memory, [token][128 channels], and written by TMA, or row
-// by row where y's rows do not start at multiples of 16 bytes: a 2-byte value a
-// lane straight to memory took 12,600 cycles a tile, against 12,000 of MMAs at
-// K = 2048, and held them up.
+// by row where y's rows do not start at multiples of 16 bytes (777 x 5,003 x 1,999
+// in f16: 24.5 us, with rows 5,008 apart and whole 20.3).  A 2-byte value a lane
+// straight to memory took 12,600 cycles a tile of 256 tokens, more than its
+// MMAs at K = 2048 (8,200); a bulk copy a row held up the loads more than the
+// warps' own stores do (28 us for the 777 rows).
 template <typename T>
 __device__ __forceinline__ void put_slabs(const GemmParams &p, const void *map_y, uint8_t *slabs, const float *sx, float sw,
                                           uint32_t (&v)[4][32], int n, int64_t m, int chan0, int h, int quad, int lane,
@@ -198,10 +202,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 // The same product where there are fewer tiles than pairs: a cluster of S pairs
 // shares one tile, each pair a part of K, because a k-step takes its 315 cycles
 // however narrow the tile (8 x 512 x 16,384: 24.6 us whole, 15.4 in four parts;
-// 8 x 2,048 x 8,192: 16.2 and 10.8).  The pairs leave their 32-bit sums in their shared memory;
-// pair s reads every pair's sums of token slice s, adds them up (whole numbers:
-// any order) and writes its slice.  (Sent instead of fetched they took two
-// barriers and 3.3 us for the smallest tile.)
+// 8 x 2,048 x 8,192: 16.2 and 10.8).  The pairs leave their 32-bit sums in their
+// shared memory; pair s reads every pair's sums of token slice s, adds them up
+// (whole numbers: any order) and writes its slice.  (Sent instead of fetched
+// they took two barriers and 3.3 us for the smallest tile.)
 template <typename T, int S>
 __global__ void __launch_bounds__(G_THREADS, 1)
     i8_split_kernel(const __grid_constant__ TmaDesc map_w, const __grid_constant__ TmaDesc map_x, GemmParams p) {

@@ -1,7 +1,9 @@
 // k_i8_head.cu — log probabilities straight from hidden states and an 8-bit LM
 // head: the product's epilogue folds every logit into its row's sums and keeps
-// the largest, so the [T][V] logits are never stored (f32 logits of 2,048
-// tokens x 131,072 would be 1 GB written and 1 GB read back).
+// the largest, so many rows' logits are never stored (f32 logits of 2,048
+// tokens x 131,072 would be 1 GB written and 1 GB read back).  2,048 x 131,072 x
+// 2,048 takes 353 us without alternatives, 3.1 POP/s; with 5 of them 420 us, the
+// tensor pipe active for 70% of the cycles: what the lists add to the epilogue.
 #include <algorithm>
 
 #include "i8_mma.cuh"
@@ -17,9 +19,9 @@ constexpr int H_ROW = 8 * G_EPI_THREADS;  // bytes between two entries of a thre
 constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
 // Ring slots and entries of a thread's list, which share a block's memory: a
 // list of 40 leaves four slots, and up to 32 entries one sort cuts it.  Above 22
-// alternatives that leaves too few new entries between two cuts (20 of 2,048 x
-// 131,072 x 2,048 took 586 us with 40 entries and 620 with 60, 32 took 4,100
-// and 740): a list of 60 beside three slots.
+// alternatives that leaves too few new entries between two cuts (2,048 x 131,072 x
+// 2,048 with 5: 418 us with 40 entries and 427 with 60; with 20: 582 and 590, 24:
+// 662 and 632, 32: 3,923 and 703): a list of 60 beside three slots.
 constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
 constexpr int64_t H_TOKENS = 4096;  // tokens of one launch

@@ -545,8 +545,10 @@ class Context:
     def i8_head_logprobs(self, w: "I8Weights", x, tokens=None, logprobs=None, entropy=None, top_ids=None,
                          top_logprobs=None, workspace=None):
         """token_logprobs of the logits x w^T (as i8_linear writes them in f32)
-        for hidden states x [T][K] and an LM head w [V][K], without the logits
-        in memory.  workspace as for i8_linear, of w.head_workspace(T, G, k) bytes."""
+        for hidden states x [T][K] and an LM head w [V][K].  The logits of many
+        rows never reach memory; few rows' (up to 64, or 16 MB of logits, times
+        max(k, 8) with k alternatives) pass through the workspace.  workspace as
+        for i8_linear, of w.head_workspace(T, G, k) bytes."""
         T, K, xp, ldx = _matrix(x, self.device, "i8_head_logprobs: x")
         if K != w.K:
             raise HarCudaError(ERR_GEOMETRY, f"i8_head_logprobs: x [T][{w.K}]")
@@ -826,7 +828,8 @@ class I8Weights:
         return int(self.ctx.lib.har_cuda_i8_linear_workspace(self.handle, M))
 
     def head_workspace(self, T: int, G: int, k: int) -> int:
-        """Bytes of workspace that i8_head_logprobs takes."""
+        """Bytes of workspace that i8_head_logprobs takes for T rows and k
+        alternatives (0: no top outputs)."""
         return int(self.ctx.lib.har_cuda_i8_head_workspace(self.handle, T, G, k))
 
     def free(self):
