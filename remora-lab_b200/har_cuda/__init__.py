@@ -1377,8 +1377,9 @@ class CudaMoeServingModel:
         -> [ScoreOutcome], one per input, in order.  The tokens are folded
         through the layers as prefill_batch folds them, sequences side by side
         (a row's step does not depend on the others'), and the head is applied
-        once, to every position of the batch: no [positions][vocab] logits with
-        an 8-bit head.  `top` alternatives a position, at most LOGPROBS_MAX_TOP."""
+        once, to every position of the batch (with an 8-bit head by
+        i8_head_logprobs, which stores no logits of many positions).  `top`
+        alternatives a position, at most LOGPROBS_MAX_TOP."""
         torch = self._torch
         seqs = [np.asarray(t, np.int64).reshape(-1) for _, t in inputs]
         if not 0 <= top <= LOGPROBS_MAX_TOP:
