@@ -185,7 +185,8 @@ int32_t har_cuda_i8_quantize(har_cuda_ctx *ctx, const void *x_dev, int32_t dtype
  * channel).  quantize: the same rule over the rows of a float matrix; the
  * handle owns its copy.  wrap: an existing device matrix, 16-byte aligned, rows
  * ldq bytes apart (a multiple of 16; bytes between K and ldq are never used),
- * not freed by the library.  Values of -128 are allowed; K <= 131,056, the
+ * not freed by the library.  quantize refuses while the stream is being captured
+ * (HAR_CUDA_ERR_ARG).  Values of -128 are allowed; K <= 131,056, the
  * longest sum that 32 bits hold. */
 int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32_t dtype,
                                      int64_t N, int64_t K, int64_t ldw,

@@ -69,6 +69,18 @@ static int32_t check_i8_weights(har_cuda_ctx *ctx, const har_cuda_i8_weights *w,
   return HAR_CUDA_OK;
 }
 
+// Whether the context's stream is being captured.
+static int32_t capturing(har_cuda_ctx *ctx, const char *who, bool *yes) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(ctx->stream, &cap);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
+  }
+  *yes = cap != cudaStreamCaptureStatusNone;
+  return HAR_CUDA_OK;
+}
+
 // `need` bytes from the caller's workspace, or from the context's arena
 // outside a capture.
 static int32_t take_workspace(har_cuda_ctx *ctx, void *ws, size_t bytes, size_t need, const char *who, uint8_t **out) {
@@ -81,16 +93,13 @@ static int32_t take_workspace(har_cuda_ctx *ctx, void *ws, size_t bytes, size_t 
     *out = (uint8_t *)ws;
     return HAR_CUDA_OK;
   }
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  const cudaError_t e = cudaStreamIsCapturing(ctx->stream, &cap);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
-  }
-  if (cap != cudaStreamCaptureStatusNone)
+  bool captured = false;
+  int32_t st = capturing(ctx, who, &captured);
+  if (st != HAR_CUDA_OK) return st;
+  if (captured)
     return set_error(ctx, HAR_CUDA_ERR_ARG, std::string(who) + ": a captured call needs a workspace of " +
                                                 std::to_string(need) + " bytes from the caller");
-  const int32_t st = ensure_scratch(ctx, need);
+  st = ensure_scratch(ctx, need);
   if (st == HAR_CUDA_OK) *out = (uint8_t *)ctx->scratch;
   return st;
 }
@@ -143,6 +152,10 @@ int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32
   HAR_TRY(check_rows(ctx, w_dev, dtype_bytes(dtype), N, K, ldw, false, "i8_weights_quantize: weights"));
   OnDevice on(ctx);
   HAR_TRY(on.status(ctx));
+  bool captured = false;
+  HAR_TRY(capturing(ctx, "i8_weights_quantize", &captured));
+  if (captured)  // the handle's memory would be written by the graph, and not before its first launch
+    return set_error(ctx, HAR_CUDA_ERR_ARG, "i8_weights_quantize: not while the stream is being captured");
   const int64_t ldq = (int64_t)round16((size_t)K);
   const size_t qb = (size_t)N * (size_t)ldq, bytes = qb + sizeof(float) * (size_t)N;
   void *d = nullptr;

@@ -356,3 +356,71 @@ def test_one_workspace_for_two_graphs_in_turn(ctx):
         torch.cuda.synchronize()
         rq, rs = quantize64(xs[i])
         assert torch.equal(ys[i].cpu(), product(rq, rs, wq, ws, torch.float32)), i
+
+
+def test_weights_are_not_made_under_capture(ctx):
+    """The handle's memory would be written by the graph; the capture goes on."""
+    x = rows(71, 5, 64)
+    w, wq, ws = weights(ctx, 72, 40, 64)
+    y = torch.zeros(5, 40, device="cuda")
+    work = torch.empty(max(16, w.linear_workspace(5)), dtype=torch.uint8, device="cuda")
+    ctx.i8_linear(w, x, y, workspace=work)
+    torch.cuda.synchronize()
+    g, side, status = torch.cuda.CUDAGraph(), torch.cuda.Stream(), None
+    try:
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            ctx.bind_torch_stream()
+            try:
+                ctx.i8_weights(x)
+            except har_cuda.HarCudaError as e:
+                status = e.status
+            ctx.i8_linear(w, x, y, workspace=work)
+            g.capture_end()
+    finally:
+        ctx.bind_torch_stream()
+    assert status == har_cuda.ERR_ARG
+    y.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y.cpu(), product(*quantize64(x), wq, ws, torch.float32))
+
+
+def test_two_contexts_share_weights(ctx):
+    """Two contexts on two streams use one handle at the same time, each with its
+    own arena; with work of every kernel in flight on both."""
+    K, N = 512, 1500
+    w, wq, ws = weights(ctx, 81, N, K)
+    other = har_cuda.Context(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    x = [rows(82, 300, K), rows(83, 300, K)]
+    sizes = (1, 7, 40, 300)
+    y = [[torch.empty(m, N, device="cuda") for m in sizes] for _ in x]
+    torch.cuda.synchronize()
+    try:
+        for i, c in enumerate((ctx, other)):
+            with torch.cuda.stream(streams[i]):
+                c.bind_torch_stream()
+        for _ in range(20):
+            for j, m in enumerate(sizes):
+                for i, c in enumerate((ctx, other)):
+                    c.i8_linear(w, x[i][:m], y[i][j])
+        torch.cuda.synchronize()
+    finally:
+        ctx.bind_torch_stream()
+    for i in range(2):
+        ref = product(*quantize64(x[i]), wq, ws, torch.float32)
+        for j, m in enumerate(sizes):
+            assert torch.equal(y[i][j].cpu(), ref[:m]), (i, m)
+    other.close()
+
+
+@pytest.mark.parametrize("M,N,K", [(1_500_007, 5, 16), (1_500_007, 129, 33), (70, 300_001, 40)])
+def test_many_rows_or_channels(ctx, M, N, K):
+    """Thousands of tiles along one side; rows from both ends and between."""
+    x = torch.randn(M, K, device="cuda", generator=torch.Generator(device="cuda").manual_seed(M))
+    w, wq, ws = weights(ctx, N, N, K)
+    y = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    ctx.i8_linear(w, x, y)
+    at = sorted({0, 1, 69, M // 3, M // 2, M - 2, M - 1} & set(range(M)))
+    assert torch.equal(y[at].cpu(), product(*quantize64(x[at]), wq, ws, torch.bfloat16))
