@@ -410,15 +410,19 @@ __global__ void __launch_bounds__(TH) head_join_kernel(const HeadJoin j) {
   __syncthreads();
   const key_t bound = bound_s;
   if (best >= bound) {
-    const int n = p.part_n[(int64_t)tid * p.Tp + t];
+    // (k at the most; a launch that gave up on a wait leaves whatever was there)
+    const int n = min(p.part_n[(int64_t)tid * p.Tp + t], p.k);
     for (int e = 0; e < n; ++e) {
       const int64_t at = ((int64_t)tid * p.k + e) * p.Tp + t;
       const key_t key = order_key(p.part_v[at], (uint32_t)p.part_i[at]);
-      if (key >= bound) cand[atomicAdd(&count, 1)] = key;
+      if (key >= bound) {
+        const int to = atomicAdd(&count, 1);
+        if (to < I8_MAX_TOP * I8_MAX_TOP) cand[to] = key;
+      }
     }
   }
   __syncthreads();
-  const int n = count;
+  const int n = min(count, I8_MAX_TOP * I8_MAX_TOP);
   key_t list = 0;
   for (int i = 32 * warp; i < n; i += TH)
     list = warp_merge_desc(list, warp_sort_desc(i + lane < n ? cand[i + lane] : (key_t)0, lane), lane);
