@@ -532,3 +532,35 @@ def test_stored_and_unstored_logits_agree(ctx):
     tol = 2 * (V / 32 * 2.0 ** -22 + 64 * 2.0 ** -24)
     for n in ("logprobs", "top"):
         assert float((many[n][100:164] - few[n]).abs().max()) <= tol, n
+
+
+@pytest.mark.parametrize("T", [2, 70])
+def test_many_given_tokens(ctx, T):
+    """More given tokens a row than a block has threads, repeated ones and
+    padding among them, from logits and from hidden states."""
+    V, K, G = 900, 48, 1000
+    w, q, s = head_of(ctx, 21, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(22)).cuda()
+    tok = given(23, T, V, G)
+    tok[:, ::7], tok[1, 500:600] = -1, 3
+    logits = product(*quantize64(x), q, s, torch.float32)
+    ref = logprobs64(logits, tok, 4)
+    got = head_score(ctx, w, x, tok, 4)
+    ctx.synchronize()
+    check_logprobs(got, ref, "head")
+    check_logprobs(score(ctx, logits.cuda(), tok, 4), ref, "logits")
+
+
+def test_many_short_rows(ctx):
+    """300,007 rows of 11 logits, and as many from hidden states."""
+    T, V, K, k = 300_007, 11, 16, 3
+    w, q, s = head_of(ctx, 24, V, K)
+    x = torch.randn(T, K, device="cuda", generator=torch.Generator(device="cuda").manual_seed(25))
+    tok = given(26, T, V, 1)
+    got = head_score(ctx, w, x, tok, k)
+    ctx.synchronize()
+    check_rows(got, q, s, x, tok, k, sample_rows(T), "head")
+    logits = torch.randn(T, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(27))
+    got = score(ctx, logits, tok, k)
+    rows = sample_rows(T)
+    check_logprobs({n: v[rows] for n, v in got.items()}, logprobs64(logits[rows], tok[rows], k), "logits")

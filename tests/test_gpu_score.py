@@ -85,3 +85,19 @@ def test_score_refuses(setup):
         model.score([(np.zeros(H, np.float32), [V])])
     with pytest.raises(har_cuda.HarCudaError):
         model.score([(np.zeros(H, np.float32), [1])], top=33)
+
+
+@pytest.mark.parametrize("head", ["i8", "q4k"])
+def test_score_without_alternatives(setup, head):
+    """top = 0: the same log probabilities and entropies, empty alternatives;
+    and nothing to score at all."""
+    model = model_of(setup, head)
+    rng = np.random.default_rng(3)
+    inputs = [(haro.normal_f32(9700 + i, 0, H, 0.0, 0.3), rng.integers(0, V, n)) for i, n in enumerate([4, 1, 0, 3])]
+    with_top, without = model.score(inputs, top=5), model.score(inputs)
+    for a, b in zip(with_top, without):
+        assert np.array_equal(a.logprobs, b.logprobs) and np.array_equal(a.entropy, b.entropy)
+        assert b.top_ids.shape == (len(b.entropy), 0) and b.top_logprobs.shape == (len(b.entropy), 0)
+    assert model.score([]) == []
+    (empty,) = model.score([(np.zeros(H, np.float32), [])], top=2)
+    assert empty.logprobs.size == 0 and empty.top_ids.shape == (0, 2)
