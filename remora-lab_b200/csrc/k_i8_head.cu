@@ -46,6 +46,7 @@ struct HeadParams {
   int32_t *part_n;                 // its entries
   float *part_v;                   // [part][k][Tp]
   int32_t *part_i;
+  uint32_t *bars;                  // [Tp]: order_bits of a value that k logits of the token reach, 0 at first
   int *status;
 };
 
@@ -112,6 +113,12 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
 #pragma unroll
   for (int j = 1; j < 32; ++j) r = j == i ? v[j] : r;
   return r;
+}
+
+__device__ __forceinline__ uint32_t ld_relaxed(const uint32_t *p) {
+  uint32_t v;
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // A thread's list in shared memory: entries (value, id), H_ROW bytes apart,
@@ -209,8 +216,21 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     float sx = 0.0f;
     int cur = -1;
 
+    // The bar that the token's parts share: each raises it to its own k-th
+    // value and lets nothing below it into its list.  It may come from any part,
+    // so a value that equals it enters still (two steps down: the one below +0 is
+    // -0, its equal); what is cut late by a bar read late is cut by the join.
+    // (128 x 131,072 x 2,048 with 5: 101 -> 95 us, 203 x 50,021 x 1,999 with 20:
+    // 103 -> 93.)
+    uint32_t seen = 0;  // as read last
+    auto share = [&](uint32_t o) {
+      if (o > seen && o > order_bits(-INFINITY) && token < p.T) atomicMax(p.bars + token, o);
+    };
     auto cut = [&](const List &l) {
-      return p.k > H_LONG ? list_cut<H_CAP_LONG - 32>(l, p.k) : list_cut<H_CAP - 32>(l, p.k);
+      List c = p.k > H_LONG ? list_cut<H_CAP_LONG - 32>(l, p.k) : list_cut<H_CAP - 32>(l, p.k);
+      if (c.bar > l.bar) share(order_bits(c.bar));
+      c.bar = fmaxf(c.bar, l.bar);
+      return c;
     };
     // the token tile's part is done
     auto flush = [&]() {
@@ -248,6 +268,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         st = {-INFINITY, 0.0f, 0.0f};
         ls.end = ls.at;
         ls.bar = token < p.T ? -INFINITY : INFINITY;
+        seen = 0;
       }
       const int64_t v0 = (int64_t)b_row + h * H_COLS;  // this half's first vocabulary row
       scales[a][h][row] = v0 + row < p.V ? __ldg(p.sw + v0 + row) : 0.0f;
@@ -297,13 +318,17 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         }
         sort32_desc(top);
         const uint32_t o = order_bits(pick32(top, p.k - 1));
-        // two steps down: the one below +0 is -0, its equal
+        share(o);
         if (token < p.T) ls.bar = order_value(max(o - 2u, order_bits(-INFINITY)));
       }
       tc::tmem_ld32(col, v);
 #pragma unroll 1
       for (int c = 0; c < H_COLS; c += 32) {
         float l[32];
+        if (p.k > 0) {
+          ls.bar = fmaxf(ls.bar, order_value(seen - 2u));  // of 0, and just above -inf, a NaN: no bar
+          if (token < p.T) seen = ld_relaxed(p.bars + token);
+        }
         logits(c, l);
         if (c + 32 < H_COLS) tc::tmem_ld32(col + (uint32_t)(c + 32), v);
         else ring_release<2>(ring, a, lane);
@@ -500,6 +525,7 @@ static size_t head_layout(const HeadPlan &h, int64_t T, int64_t K, int k, uint8_
     p.part_n = (int32_t *)take(sizeof(int32_t) * cells);
     p.part_v = (float *)take(sizeof(float) * cells * (size_t)k);
     p.part_i = (int32_t *)take(sizeof(int32_t) * cells * (size_t)k);
+    p.bars = (uint32_t *)take(sizeof(uint32_t) * (size_t)h.Tp);
   }
   return n;
 }
@@ -514,11 +540,9 @@ static int64_t head_chunk(int64_t T) {
 // tokens, of which a tile of 256 makes little (64 x 131,072 x 4,096: 110 us against
 // 118), and where the lists that every part of a row keeps cost more than the
 // logits' way: that grows with the alternatives.  For 256 x 131,072 x 2,048 the
-// walk takes 110 to 115 us, this kernel 72, 89, 95, 105, 114, 121 and 149 with 0, 1,
-// 2, 5, 8, 12 and 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 63, 67, 72
-// (5) and 103 (20); for 2,048 x 32,000 x 2,048 170 (8), 176 (20) and 187 (32),
-// and 164, 229 and 300; for 768 x 131,072 x 2,048 252 (8), 254 and 262, and 218,
-// 293 and 378.
+// walk takes 110 to 115 us, this kernel 72, 85, 98, 106 and 142 with 0, 1, 5, 8 and
+// 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 61, 66 (5) and 93 (20);
+// for 768 x 131,072 x 2,048 252 (8), 254 (20) and 262 (32), and 207, 279 and 363.
 static bool head_walks(int64_t T, int64_t V, int k) {
   return T <= H_WALK_TOKENS || T * V * (int64_t)sizeof(float) <= (k ? std::max(k, 8) : 1) * H_WALK_BYTES;
 }
@@ -586,6 +610,8 @@ int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     TmaDesc map_x;
     st = encode_tmap_2d(ctx, &map_x, q, 1, (uint64_t)n, (uint64_t)w->K, (uint64_t)ldq, G_A, G_KS, true);
     if (st != HAR_CUDA_OK) return st;
+    if (k > 0 && cudaMemsetAsync(p.bars, 0, sizeof(uint32_t) * (size_t)h.Tp, ctx->stream) != cudaSuccess)
+      return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_logprobs: ") + cudaGetErrorString(cudaGetLastError()));
     const size_t smem = (size_t)p.sh.stages * H_SLOT + (size_t)cap * H_ROW + 1024;
     prof_begin(ctx);
     const cudaError_t e = launch_clusters(i8_head_kernel, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 2, map_x, w->map, p);
