@@ -238,7 +238,7 @@ int32_t har_cuda_token_logprobs(har_cuda_ctx *ctx, const void *logits_dev, int32
                                 int32_t *top_ids_dev, float *top_logprobs_dev);
 /* har_cuda_token_logprobs of the logits that har_cuda_i8_linear would write as
  * f32 for the LM head w [V][K] and hidden states x_dev [T][K].  The logits of
- * many rows never reach memory; those of up to 64 rows, and up to 16 MB of them
+ * many rows never reach memory; those of up to 64 rows, and up to 12 MB of them
  * (times max(k, 8) with alternatives), pass through the workspace, where that is
  * faster.  Workspace as for har_cuda_i8_linear, of har_cuda_i8_head_workspace
  * bytes for this T and k (one for k serves k = 0 too). */

@@ -2,8 +2,8 @@
 // head: the product's epilogue folds every logit into its row's sums and keeps
 // the largest, so many rows' logits are never stored (f32 logits of 2,048
 // tokens x 131,072 would be 1 GB written and 1 GB read back).  2,048 x 131,072 x
-// 2,048 takes 353 us without alternatives, 3.1 POP/s; with 5 of them 420 us, the
-// tensor pipe active for 70% of the cycles: what the lists add to the epilogue.
+// 2,048 takes 350 us without alternatives, 3.1 POP/s, and 376 with 5 of them, what
+// the lists add to the epilogue.
 #include <algorithm>
 
 #include "i8_mma.cuh"
@@ -20,12 +20,13 @@ constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
 // Ring slots and entries of a thread's list, which share a block's memory: a
 // list of 40 leaves four slots, and up to 32 entries one sort cuts it.  Above 22
 // alternatives that leaves too few new entries between two cuts (2,048 x 131,072 x
-// 2,048 with 5: 418 us with 40 entries and 427 with 60; with 20: 582 and 590, 24:
-// 662 and 632, 32: 3,923 and 703): a list of 60 beside three slots.
+// 2,048 with 5: 384 us with 40 entries and 405 with 60; with 20: 445 and 449, 24:
+// 500 and 466, 32: 3,148 and 604): a list of 60 beside three slots.
 constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
+constexpr int H_PEERS = 16;  // parts that a part asks
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
 constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
-constexpr int64_t H_WALK_TOKENS = 64, H_WALK_BYTES = 16 << 20;
+constexpr int64_t H_WALK_TOKENS = 64, H_WALK_BYTES = 12 << 20;
 
 struct HeadPlan {
   int tt, vt, g, C, passes;         // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
@@ -46,7 +47,7 @@ struct HeadParams {
   int32_t *part_n;                 // its entries
   float *part_v;                   // [part][k][Tp]
   int32_t *part_i;
-  uint32_t *bars;                  // [Tp]: order_bits of a value that k logits of the token reach, 0 at first
+  uint64_t *best2;                 // [part][Tp]: order_bits of two of its logits, 0 at first
   int *status;
 };
 
@@ -75,14 +76,15 @@ struct HeadTiles {
   }
 };
 
-// 32 values a thread in descending order (bitonic, in registers).
-__device__ __forceinline__ void sort32_desc(float (&v)[32]) {
+// N values (a power of two) a thread in descending order (bitonic, in registers).
+template <int N>
+__device__ __forceinline__ void sort_desc(float (&v)[N]) {
 #pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
+  for (int size = 2; size <= N; size <<= 1)
 #pragma unroll
     for (int step = size >> 1; step > 0; step >>= 1)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int j = i ^ step;
         if (j > i) {
           const float hi = fmaxf(v[i], v[j]), lo = fminf(v[i], v[j]);
@@ -108,17 +110,39 @@ __device__ __forceinline__ void merge32_desc(float (&a)[32], const float (&b)[32
       }
     }
 }
-__device__ __forceinline__ float pick32(const float (&v)[32], int i) {
+template <int N>
+__device__ __forceinline__ float pick(const float (&v)[N], int i) {
   float r = v[0];
 #pragma unroll
-  for (int j = 1; j < 32; ++j) r = j == i ? v[j] : r;
+  for (int j = 1; j < N; ++j) r = j == i ? v[j] : r;
   return r;
 }
 
-__device__ __forceinline__ uint32_t ld_relaxed(const uint32_t *p) {
-  uint32_t v;
-  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
+// The parts of a token tell each other their two largest logits so far.  The
+// k-th largest of what H_PEERS of them tell bounds the k-th largest of all from below, and far closer than a
+// part's own k-th: 1 or 2 of the logits that a part has seen reach it, not k.
+// Both in one word: the first of one telling and the second of a later one may
+// be the same logit.
+__device__ __forceinline__ void tell_best2(uint64_t *at, float a, float b) {
+  const uint64_t two = ((uint64_t)order_bits(b) << 32) | order_bits(a);
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(at), "l"(two) : "memory");
+}
+// A float just below that bound: what equals it may have the lower id.
+__device__ __noinline__ float peers_bar(const uint64_t *best2, int64_t Tp, int part, int parts, int k) {
+  float v[2 * H_PEERS];
+#pragma unroll
+  for (int i = 0; i < H_PEERS; ++i) {
+    uint64_t two = 0;
+    const int p = part + i < parts ? part + i : part + i - parts;
+    if (i < parts)
+      asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(two) : "l"(best2 + p * Tp) : "memory");
+    const uint32_t a = (uint32_t)two, b = (uint32_t)(two >> 32);
+    v[2 * i] = a ? order_value(a) : -INFINITY;
+    v[2 * i + 1] = b ? order_value(b) : -INFINITY;
+  }
+  sort_desc(v);
+  // two steps down: the one below +0 is -0, its equal; of -inf a NaN, no bar
+  return order_value(order_bits(pick(v, k - 1)) - 2u);
 }
 
 // A thread's list in shared memory: entries (value, id), H_ROW bytes apart,
@@ -160,16 +184,16 @@ __device__ __noinline__ List list_cut(List s, int k) {
   const int n = s.n();
 #pragma unroll
   for (int i = 0; i < 32; ++i) top[i] = i < n ? list_value(s.at + i * H_ROW) : -INFINITY;
-  sort32_desc(top);
+  sort_desc(top);
   if (__any_sync(0xffffffffu, n > 32)) {
     float more[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) more[i] = i < MORE && 32 + i < n ? list_value(s.at + (32 + i) * H_ROW) : -INFINITY;
-    sort32_desc(more);
+    sort_desc(more);
     merge32_desc(top, more);
   }
   if (n < k) return s;
-  const float bar = pick32(top, k - 1);
+  const float bar = pick(top, k - 1);
   int equals = k;
 #pragma unroll
   for (int i = 0; i < 32; ++i) equals -= i < k && top[i] > bar;
@@ -216,21 +240,26 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     float sx = 0.0f;
     int cur = -1;
 
-    // The bar that the token's parts share: each raises it to its own k-th
-    // value and lets nothing below it into its list.  It may come from any part,
-    // so a value that equals it enters still (two steps down: the one below +0 is
-    // -0, its equal); what is cut late by a bar read late is cut by the join.
-    // (128 x 131,072 x 2,048 with 5: 101 -> 95 us, 203 x 50,021 x 1,999 with 20:
-    // 103 -> 93.)
-    uint32_t seen = 0;  // as read last
-    auto share = [&](uint32_t o) {
-      if (o > seen && o > order_bits(-INFINITY) && token < p.T) atomicMax(p.bars + token, o);
-    };
+    const int mine = 2 * tiles.c + h;  // this thread's part
+    int walked = 0;                    // tiles of the token tile so far
     auto cut = [&](const List &l) {
       List c = p.k > H_LONG ? list_cut<H_CAP_LONG - 32>(l, p.k) : list_cut<H_CAP - 32>(l, p.k);
-      if (c.bar > l.bar) share(order_bits(c.bar));
-      c.bar = fmaxf(c.bar, l.bar);
+      c.bar = fmaxf(c.bar, l.bar);  // the peers' may be higher
       return c;
+    };
+    // after 1, 2, 4, ... tiles: tells the list's two largest, and learns (2,048 x
+    // 131,072 x 2,048 with 5, 20 and 32: 418, 575 and 704 us without, 376, 460 and
+    // 610 with it; 768 tokens with 8 and 20: 218 and 293, 188 and 234)
+    auto confer = [&]() {
+      float a = -INFINITY, b = -INFINITY;
+      for (uint32_t e = ls.at; e < ls.end; e += H_ROW) {
+        const float x = list_value(e);
+        b = fmaxf(b, fminf(a, x));
+        a = fmaxf(a, x);
+      }
+      if (token >= p.T) return;
+      if (b > -INFINITY) tell_best2(p.best2 + mine * p.Tp + token, a, b);
+      ls.bar = fmaxf(ls.bar, peers_bar(p.best2 + token, p.Tp, mine, 2 * p.C, p.k));
     };
     // the token tile's part is done
     auto flush = [&]() {
@@ -268,7 +297,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         st = {-INFINITY, 0.0f, 0.0f};
         ls.end = ls.at;
         ls.bar = token < p.T ? -INFINITY : INFINITY;
-        seen = 0;
+        walked = 0;
       }
       const int64_t v0 = (int64_t)b_row + h * H_COLS;  // this half's first vocabulary row
       scales[a][h][row] = v0 + row < p.V ? __ldg(p.sw + v0 + row) : 0.0f;
@@ -316,19 +345,19 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           for (int i = 0; i < 32; i += 4)
             top[(c + i) / 4] = fmaxf(fmaxf(fmaxf(l[i], l[i + 1]), fmaxf(l[i + 2], l[i + 3])), -INFINITY);
         }
-        sort32_desc(top);
-        const uint32_t o = order_bits(pick32(top, p.k - 1));
-        share(o);
+        sort_desc(top);
+        const uint32_t o = order_bits(pick(top, p.k - 1));
+        if (token < p.T && top[1] > -INFINITY) tell_best2(p.best2 + mine * p.Tp + token, top[0], top[1]);
         if (token < p.T) ls.bar = order_value(max(o - 2u, order_bits(-INFINITY)));
+      }
+      if (p.k > 0) {
+        if (walked > 0 && (walked & (walked - 1)) == 0) confer();
+        ++walked;
       }
       tc::tmem_ld32(col, v);
 #pragma unroll 1
       for (int c = 0; c < H_COLS; c += 32) {
         float l[32];
-        if (p.k > 0) {
-          ls.bar = fmaxf(ls.bar, order_value(seen - 2u));  // of 0, and just above -inf, a NaN: no bar
-          if (token < p.T) seen = ld_relaxed(p.bars + token);
-        }
         logits(c, l);
         if (c + 32 < H_COLS) tc::tmem_ld32(col + (uint32_t)(c + 32), v);
         else ring_release<2>(ring, a, lane);
@@ -525,7 +554,7 @@ static size_t head_layout(const HeadPlan &h, int64_t T, int64_t K, int k, uint8_
     p.part_n = (int32_t *)take(sizeof(int32_t) * cells);
     p.part_v = (float *)take(sizeof(float) * cells * (size_t)k);
     p.part_i = (int32_t *)take(sizeof(int32_t) * cells * (size_t)k);
-    p.bars = (uint32_t *)take(sizeof(uint32_t) * (size_t)h.Tp);
+    p.best2 = (uint64_t *)take(sizeof(uint64_t) * cells);
   }
   return n;
 }
@@ -540,9 +569,9 @@ static int64_t head_chunk(int64_t T) {
 // tokens, of which a tile of 256 makes little (64 x 131,072 x 4,096: 110 us against
 // 118), and where the lists that every part of a row keeps cost more than the
 // logits' way: that grows with the alternatives.  For 256 x 131,072 x 2,048 the
-// walk takes 110 to 115 us, this kernel 72, 85, 98, 106 and 142 with 0, 1, 5, 8 and
-// 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 61, 66 (5) and 93 (20);
-// for 768 x 131,072 x 2,048 252 (8), 254 (20) and 262 (32), and 207, 279 and 363.
+// walk takes 110 to 115 us, this kernel 72, 100, 101, 106 and 135 with 0, 1, 5, 8 and
+// 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 67, 72 (5) and 99 (20);
+// for 768 x 131,072 x 2,048 252 (8), 254 (20) and 262 (32), and 188, 234 and 322.
 static bool head_walks(int64_t T, int64_t V, int k) {
   return T <= H_WALK_TOKENS || T * V * (int64_t)sizeof(float) <= (k ? std::max(k, 8) : 1) * H_WALK_BYTES;
 }
@@ -610,7 +639,7 @@ int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     TmaDesc map_x;
     st = encode_tmap_2d(ctx, &map_x, q, 1, (uint64_t)n, (uint64_t)w->K, (uint64_t)ldq, G_A, G_KS, true);
     if (st != HAR_CUDA_OK) return st;
-    if (k > 0 && cudaMemsetAsync(p.bars, 0, sizeof(uint32_t) * (size_t)h.Tp, ctx->stream) != cudaSuccess)
+    if (k > 0 && cudaMemsetAsync(p.best2, 0, sizeof(uint64_t) * (size_t)h.parts() * (size_t)h.Tp, ctx->stream) != cudaSuccess)
       return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_logprobs: ") + cudaGetErrorString(cudaGetLastError()));
     const size_t smem = (size_t)p.sh.stages * H_SLOT + (size_t)cap * H_ROW + 1024;
     prof_begin(ctx);

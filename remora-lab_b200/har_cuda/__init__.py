@@ -546,7 +546,7 @@ class Context:
                          top_logprobs=None, workspace=None):
         """token_logprobs of the logits x w^T (as i8_linear writes them in f32)
         for hidden states x [T][K] and an LM head w [V][K].  The logits of many
-        rows never reach memory; few rows' (up to 64, or 16 MB of logits, times
+        rows never reach memory; few rows' (up to 64, or 12 MB of logits, times
         max(k, 8) with k alternatives) pass through the workspace.  workspace as
         for i8_linear, of w.head_workspace(T, G, k) bytes."""
         T, K, xp, ldx = _matrix(x, self.device, "i8_head_logprobs: x")

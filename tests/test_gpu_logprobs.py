@@ -360,13 +360,13 @@ def test_head_scales_that_are_not_numbers(ctx, T):
 
 # ---- from hidden states, where the logits are not stored ------------------------------
 #
-# More than 64 tokens and more than 16 MB of logits, times the alternatives: the
+# More than 64 tokens and more than 12 MB of logits, times the alternatives: the
 # product's epilogue keeps the sums and the lists.  A sample of rows is checked:
 # both ends, the joints between tiles of 128 and 256 tokens, and the special ones.
 
 
 def unstored(T, V, k):
-    return T > 64 and 4 * T * V > (max(k, 8) if k else 1) * 2 ** 24
+    return T > 64 and 4 * T * V > (max(k, 8) if k else 1) * 12 * 2 ** 20
 
 
 def sample_rows(T):
