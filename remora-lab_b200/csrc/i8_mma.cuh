@@ -40,21 +40,17 @@ struct RingShape {
 };
 inline int ksteps_of(int64_t K) { return (int)((K + G_KS - 1) / G_KS); }
 
-__device__ __forceinline__ bool g_wait(uint64_t *bar, uint32_t parity, volatile int *abort_s, uint32_t sleep_ns = 0) {
-  if (*abort_s) return false;
-  if (sleep_ns ? tc::mbar_wait_lazy(bar, parity, G_WAIT_LIMIT, sleep_ns) : tc::mbar_wait(bar, parity, G_WAIT_LIMIT))
-    return true;
-  *abort_s = 1;
-  return false;
-}
+// A whole warp, lane 0 between polls asleep for up to sleep_ns.
 __device__ __forceinline__ bool g_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_s, int lane,
-                                            uint32_t sleep_ns = 0) {
+                                            uint32_t sleep_ns) {
   if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity))) return true;
   bool ok = true;
-  if (lane == 0) ok = g_wait(bar, parity, abort_s, sleep_ns);
+  if (lane == 0) {
+    ok = !*abort_s && tc::mbar_wait_lazy(bar, parity, G_WAIT_LIMIT, sleep_ns);
+    if (!ok) *abort_s = 1;
+  }
   return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
-
 // The same for the roles that feed the tensor core: every step of it decided by
 // a vote, so that the loop around it stays uniform and its descriptors,
 // addresses and counters in uniform registers (see elect_one).

@@ -29,12 +29,6 @@ __device__ __forceinline__ void stat_move(Stat &a, float r) {
   a.s = f * a.s;
   a.r = r;
 }
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
-  const float r = fmaxf(a.r, b.r);
-  stat_move(a, r);
-  stat_move(b, r);
-  return {r, a.s + b.s, a.t + b.t};
-}
 __device__ __forceinline__ Stat warp_stat(Stat a) {
   stat_move(a, order_value(__reduce_max_sync(0xffffffffu, order_bits(a.r))));
 #pragma unroll

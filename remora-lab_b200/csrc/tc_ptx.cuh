@@ -283,17 +283,10 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
-// TMA load into this CTA's shared memory that completes on a barrier of either
-// CTA of the pair (a mapped address).  No multicast.
-__device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *tmap, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(tmap), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-// The same loads, and the arrival that announces their bytes, by the lane of a
-// whole warp whose `lead` is not 0: see elect_one.
+// TMA loads, and the arrival that announces their bytes, by the lane of a whole
+// warp whose `lead` is not 0: see elect_one.  The pair's load into this CTA's
+// shared memory completes on a barrier of either CTA (a mapped address).  No
+// multicast.
 __device__ __forceinline__ void tma_load_2d_w(uint32_t lead, uint32_t dst, const void *tmap, int x, int y, uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\t"
