@@ -8,7 +8,7 @@
 namespace har {
 
 constexpr int V_T = 512, V_WARPS = V_T / 32, V_R = 2, V_UN = 2;
-constexpr int V_MAX_SMEM = 96 * 1024;
+constexpr int V_MAX_SMEM = 24 * 1024;
 
 struct GemvParams {
   const int8_t *w;
@@ -177,11 +177,13 @@ __global__ void __launch_bounds__(V_T, 2) i8_gemv_kernel(const GemvParams p) {
 
 static int gemv_rows(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
 
-// Up to 4 rows, and 8 of a small matrix: above, the tensor cores' launch and its
-// quantising pass cost less than quantising the rows in every block and a dp4a
-// a row and four bytes (131,072 x 4,096: 80 us here and 91 there for 2 rows, 96 and
-// 91 for 4; 4,096 x 2,048: 8.3 and 13.7 for 4 rows, 10.6 and 12.9 for 8;
-// 4,096 x 4,096: 16.6 and 15.0 for 8).
+// Up to 4 rows, and 8 of a small matrix, that take 24 KB: above, the tensor cores'
+// launch and its quantising pass cost less than quantising the rows in every
+// block and a dp4a a row and four bytes.  Here and there, us: 131,072 x 4,096 with
+// 2 rows 80 and 91, 4 rows 96 and 91; 4,096 x 2,048 with 4 rows 8.2 and 12.3, 8
+// rows 10.3 and 12.3; 8 rows of 65,536 x 2,048 47 and 31; 512 x 4,096 with 4 rows
+// 10.3 and 12.3, 8 rows 16.4 and 12.3; 1,024 x 16,384 with one row 18.5 and 19.5, 2
+// rows 22.6 and 19.5.
 bool i8_gemv_takes(int64_t M, int64_t N, int64_t K) {
   return (M <= 4 || (M <= 8 && N * K <= 8 << 20)) && gemv_rows(M) * ((K + 15) / 16 * 16) <= V_MAX_SMEM;
 }
@@ -197,11 +199,7 @@ int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
   const size_t smem = (size_t)mt * (size_t)((w->K + 15) / 16 * 16);
   const int64_t blocks = (w->N + V_WARPS * V_R - 1) / (V_WARPS * V_R);
   const unsigned grid = (unsigned)std::min<int64_t>(blocks, 2 * ctx->num_sms);
-  cudaError_t e = cudaSuccess;
-  auto go = [&](auto kernel) {
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, V_MAX_SMEM);
-    if (e == cudaSuccess) kernel<<<grid, V_T, smem, ctx->stream>>>(p);
-  };
+  auto go = [&](auto kernel) { kernel<<<grid, V_T, smem, ctx->stream>>>(p); };
   prof_begin(ctx);
   with_dtype(y_dtype, [&](auto t) {
     using T = decltype(t);
@@ -210,10 +208,7 @@ int32_t launch_i8_gemv(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     else if (mt == 4) go(i8_gemv_kernel<T, 4>);
     else go(i8_gemv_kernel<T, 8>);
   });
-  const int32_t st = check_launch(ctx, "i8_gemv_kernel");
-  if (e != cudaSuccess)
-    return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_gemv_kernel: ") + cudaGetErrorString(e));
-  return st;
+  return check_launch(ctx, "i8_gemv_kernel");
 }
 
 }  // namespace har

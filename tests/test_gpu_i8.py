@@ -115,7 +115,10 @@ SHAPES = [(1, 1, 1), (1, 3, 16), (1, 130, 2048), (2, 64, 15), (3, 127, 17), (4, 
           (257, 256, 4096), (300, 1031, 777), (513, 260, 1024), (700, 5, 33), (1025, 515, 160), (2050, 1300, 720), (513, 5003, 96), (4100, 300, 48), (16, 1000, 2048),
           (100, 700, 1153), (512, 1500, 1100), (40, 3000, 600),
           # 5 to 8 rows: of a small matrix, of one just too large, with the longest rows on either side
-          (5, 1, 1), (6, 1000, 2051), (8, 4096, 2048), (8, 8200, 1100), (5, 3, 12285), (8, 70, 12300)]
+          (5, 1, 1), (6, 1000, 2051), (8, 4096, 2048), (8, 8200, 1100), (5, 3, 12285), (8, 70, 12300),
+          # the longest rows that a block keeps, and longer ones
+          (8, 40, 3060), (8, 40, 3080), (4, 70, 6140), (4, 70, 6150), (2, 33, 12280), (2, 33, 12300),
+          (1, 9, 24570), (1, 9, 24580)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
