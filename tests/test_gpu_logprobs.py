@@ -564,3 +564,22 @@ def test_many_short_rows(ctx):
     got = score(ctx, logits, tok, k)
     rows = sample_rows(T)
     check_logprobs({n: v[rows] for n, v in got.items()}, logprobs64(logits[rows], tok[rows], k), "logits")
+
+
+def test_workspace_for_alternatives_serves_none(ctx):
+    """A workspace of head_workspace(T, G, k) bytes holds a call without
+    alternatives too, on either side of the sizes where the logits are stored."""
+    for V in (3, 700, 40_000, 131_072):
+        w, q, s = head_of(ctx, V, V, 32)
+        for T in (1, 4, 5, 64, 65, 90, 257, 700, 4096, 4097, 9001):
+            for k in (1, 8, 9, 32):
+                assert 0 <= w.head_workspace(T, 1, 0) <= w.head_workspace(T, 1, k), (T, V, k)
+    T, V = 130, 40_000
+    w, q, s = head_of(ctx, 31, V, 32)
+    x = torch.randn(T, 32, generator=torch.Generator().manual_seed(32)).cuda()
+    tok = given(33, T, V, 1)
+    work = torch.empty(w.head_workspace(T, 1, 5), dtype=torch.uint8, device="cuda")
+    o = outputs(T, 1, 0)
+    ctx.i8_head_logprobs(w, x, tok, o["logprobs"], o["entropy"], workspace=work)
+    ctx.synchronize()
+    check_rows(o, q, s, x, tok, 0, sample_rows(T), "none")
