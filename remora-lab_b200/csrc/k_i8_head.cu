@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       uint32_t v[32];
       // 32 logits from column c on, as i8_linear writes them; -inf past V
       auto logits = [&](int c, float (&l)[32]) {
+        __syncwarp();  // lists grow and are cut lane by lane
         tc::tmem_wait_ld32(v);
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -354,6 +355,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         if (walked > 0 && (walked & (walked - 1)) == 0) confer();
         ++walked;
       }
+      // lanes past T told and asked nothing: the warp is whole again before
+      // tcgen05.ld, which all its lanes execute together
+      __syncwarp();
       tc::tmem_ld32(col, v);
 #pragma unroll 1
       for (int c = 0; c < H_COLS; c += 32) {

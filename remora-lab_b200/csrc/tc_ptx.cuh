@@ -130,8 +130,10 @@ template <int N>
 __device__ __forceinline__ void bulk_wait() {
   asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
 }
-// Barrier `id` (1 to 15) among `threads` threads, whole warps.
+// Barrier `id` (1 to 15) among `threads` threads, whole warps.  bar.sync is
+// .aligned: a warp arrives as one, so lanes that went separate ways rejoin first.
 __device__ __forceinline__ void bar_sync(int id, int threads) {
+  __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 

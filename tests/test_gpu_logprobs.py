@@ -583,3 +583,16 @@ def test_workspace_for_alternatives_serves_none(ctx):
     ctx.i8_head_logprobs(w, x, tok, o["logprobs"], o["entropy"], workspace=work)
     ctx.synchronize()
     check_rows(o, q, s, x, tok, 0, sample_rows(T), "none")
+
+
+@pytest.mark.parametrize("T,k", [(257, 5), (129, 3), (225, 24), (290, 12)])
+def test_large_head_with_few_tokens_in_the_last_warps(ctx, T, k):
+    """A token tile with one to three live lanes in its last warp, over enough
+    vocabulary tiles that its parts confer several times: lanes past T skip what
+    the others do between two of the warp's reads of tensor memory."""
+    V, K = 420_001, 16
+    w, q, s = head_of(ctx, 41 + k, V, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(T)).cuda()
+    tok = given(42, T, V, 1)
+    rows = sorted({0, 127, 128, T // 2, 160, T - 3, T - 2, T - 1} & set(range(T)))
+    check_large_head(ctx, w, q, s, x, tok, k, rows=rows, what=(T, k))
