@@ -183,11 +183,13 @@ int32_t har_cuda_i8_quantize(har_cuda_ctx *ctx, const void *x_dev, int32_t dtype
                              float *scale_dev);
 /* A weight matrix [N][K] in 8-bit integers with one scale per row (output
  * channel).  quantize: the same rule over the rows of a float matrix; the
- * handle owns its copy.  wrap: an existing device matrix, 16-byte aligned, rows
- * ldq bytes apart (a multiple of 16; bytes between K and ldq are never used),
- * not freed by the library.  quantize refuses while the stream is being captured
- * (HAR_CUDA_ERR_ARG).  Values of -128 are allowed; K <= 131,056, the
- * longest sum that 32 bits hold. */
+ * handle owns its copy, which is written when the call returns (it waits for the
+ * context's stream), so any context of the device can use it on any stream.
+ * wrap: an existing device matrix, 16-byte aligned, rows ldq bytes apart (a
+ * multiple of 16; bytes between K and ldq are never used), not freed by the
+ * library; the caller orders its writes before the calls that read it.  quantize
+ * refuses while the stream is being captured (HAR_CUDA_ERR_ARG).  Values of -128
+ * are allowed; K <= 131,056, the longest sum that 32 bits hold. */
 int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32_t dtype,
                                      int64_t N, int64_t K, int64_t ldw,
                                      har_cuda_i8_weights **out);

@@ -163,7 +163,16 @@ int32_t har_cuda_i8_weights_quantize(har_cuda_ctx *ctx, const void *w_dev, int32
     cudaGetLastError();
     return set_error(ctx, HAR_CUDA_ERR_OOM, "i8_weights_quantize: cudaMalloc of " + std::to_string(bytes) + " bytes failed");
   }
-  const int32_t st = launch_i8_quantize(ctx, w_dev, dtype, N, K, ldw, (int8_t *)d, ldq, (float *)((uint8_t *)d + qb));
+  int32_t st = launch_i8_quantize(ctx, w_dev, dtype, N, K, ldw, (int8_t *)d, ldq, (float *)((uint8_t *)d + qb));
+  // any context of the device may use the handle, on any stream: it is filled
+  // before it is given out, as uploaded weights are
+  if (st == HAR_CUDA_OK) {
+    const cudaError_t e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      st = set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_weights_quantize: ") + cudaGetErrorString(e));
+    }
+  }
   if (st != HAR_CUDA_OK) {
     cudaFree(d);
     return st;

@@ -460,7 +460,7 @@ class Context:
 
     def i8_weights(self, w) -> "I8Weights":
         """A float matrix [N][K] on the device as 8-bit integers with a scale
-        per row, in memory of the handle's own."""
+        per row, in memory of the handle's own, written when the call returns."""
         N, K, wp, ldw = _matrix(w, self.device, "i8_weights")
         h = C.c_void_p()
         self.check(self.lib.har_cuda_i8_weights_quantize(self.handle, wp, _dtype(w, "i8_weights"), N, K,

@@ -427,3 +427,33 @@ def test_many_rows_or_channels(ctx, M, N, K):
     ctx.i8_linear(w, x, y)
     at = sorted({0, 1, 69, M // 3, M // 2, M - 2, M - 1} & set(range(M)))
     assert torch.equal(y[at].cpu(), product(*quantize64(x[at]), wq, ws, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_new_weights_are_ready_for_any_stream(ctx, dtype):
+    """Weights made behind long work on one stream, multiplied at once by another
+    context on another: the handle is filled when the call returns."""
+    N, K = 700, 512
+    source, x = rows(91, N, K, dtype), rows(92, 40, K)
+    other = har_cuda.Context(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    y = [torch.empty(m, N, device="cuda") for m in (1, 40)]
+    big = torch.randn(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(streams[0]):
+            ctx.bind_torch_stream()
+            for _ in range(20):
+                big = big @ big * 1e-2
+            w = ctx.i8_weights(source)
+        with torch.cuda.stream(streams[1]):
+            other.bind_torch_stream()
+            for out in y:
+                other.i8_linear(w, x[:out.shape[0]], out)
+        torch.cuda.synchronize()
+    finally:
+        ctx.bind_torch_stream()
+    ref = product(*quantize64(x), *quantize64(source), torch.float32)
+    for out in y:
+        assert torch.equal(out.cpu(), ref[:out.shape[0]]), out.shape
+    other.close()
