@@ -84,7 +84,9 @@ int32_t har_cuda_ctx_destroy(har_cuda_ctx *ctx);
 int32_t har_cuda_last_error(const har_cuda_ctx *ctx, char *buf, size_t len);
 /* Launch on a caller-owned cudaStream_t (NULL restores the context's own,
  * a non-blocking stream; pass cudaStreamLegacy, 0x1, to run on the legacy
- * default stream and order with other default-stream work). */
+ * default stream and order with other default-stream work).  Routing and the
+ * MoE layers keep intermediate results in one arena of the context: the caller
+ * orders a new stream behind such calls on the stream before. */
 int32_t har_cuda_ctx_set_stream(har_cuda_ctx *ctx, void *cuda_stream);
 /* Experts with at least `min_tokens` tokens in a moe_ffn call run on the
  * tensor-core (tcgen05) kernels, the rest on the CUDA-core GEMV kernels;
@@ -208,10 +210,13 @@ int32_t har_cuda_i8_matmul(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
 /* The same from float rows: quantises x_dev [M][K] (rows ldx elements apart)
  * and multiplies; bit for bit har_cuda_i8_quantize followed by
  * har_cuda_i8_matmul.  The quantised rows live in workspace_dev (16-byte
- * aligned, at least har_cuda_i8_linear_workspace(w, M) bytes), or with NULL in
- * the context's scratch arena.  While the stream is being captured a call that
- * needs workspace takes it from the caller only (HAR_CUDA_ERR_ARG with NULL): a
- * graph must not keep an address that a later call may free. */
+ * aligned, at least har_cuda_i8_linear_workspace(w, M) bytes), or with NULL in a
+ * workspace of the context's own.  That one is used in order: a call on another
+ * stream than the last waits on the device until the last is done with it, so
+ * work that is to overlap on two streams brings workspaces.  While the stream is
+ * being captured a call that needs workspace takes it from the caller only
+ * (HAR_CUDA_ERR_ARG with NULL): a graph must not keep an address that a later
+ * call may free. */
 int64_t har_cuda_i8_linear_workspace(const har_cuda_i8_weights *w, int64_t M);
 int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const void *x_dev,
                            int32_t x_dtype, int64_t ldx, int64_t M, void *y_dev, int32_t y_dtype,

@@ -182,6 +182,7 @@ int32_t har_cuda_ctx_destroy(har_cuda_ctx *ctx) {
   prof_clear(ctx);
   if (ctx->host_graph.exec) cudaGraphExecDestroy(ctx->host_graph.exec);
   if (ctx->scratch) cudaFree(ctx->scratch);
+  free_workspace(ctx);
   if (ctx->host_pinned) cudaFreeHost(ctx->host_pinned);
   if (ctx->io_dev) cudaFree(ctx->io_dev);
   if (ctx->d_status) cudaFree(ctx->d_status);

@@ -231,6 +231,16 @@ struct har_cuda_ctx {
   size_t host_pinned_bytes = 0;
   void *io_dev = nullptr;             // device staging for *_host entry points
   size_t io_dev_bytes = 0;
+  // workspace of the 8-bit products and the head scoring (score.cu), apart from
+  // the scratch arena: the streams that a context is bound to in turn are ordered
+  // over it
+  struct Workspace {
+    void *p = nullptr;
+    size_t bytes = 0;
+    cudaStream_t stream = nullptr;  // of its last use, with the process-unique id
+    unsigned long long stream_id = 0;
+    cudaEvent_t used = nullptr;     // behind the last use
+  } ws;
   int64_t launches = 0;
   int tc_min_tokens = 0;              // tensor-core threshold override (0 = default)
   uint64_t epoch = 0;                 // bumped whenever scratch or staging is reallocated
@@ -317,6 +327,8 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 int32_t ensure_scratch(har_cuda_ctx *ctx, size_t bytes);
+// Frees ctx->ws once its last use is over.
+void free_workspace(har_cuda_ctx *ctx);
 
 // Kernel launchers (host functions defined in the kernel .cu files).
 int32_t launch_q8k_quantize(har_cuda_ctx *ctx, const float *x, int64_t M, int64_t K,

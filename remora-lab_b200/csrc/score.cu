@@ -81,28 +81,90 @@ static int32_t capturing(har_cuda_ctx *ctx, const char *who, bool *yes) {
   return HAR_CUDA_OK;
 }
 
-// `need` bytes from the caller's workspace, or from the context's arena
-// outside a capture.
-static int32_t take_workspace(har_cuda_ctx *ctx, void *ws, size_t bytes, size_t need, const char *who, uint8_t **out) {
-  *out = nullptr;
-  if (need == 0) return HAR_CUDA_OK;
-  if (ws) {
-    if (((uintptr_t)ws & 15u) || bytes < need)
-      return set_error(ctx, HAR_CUDA_ERR_ARG, std::string(who) + ": the workspace must be 16-byte aligned and hold " +
-                                                  std::to_string(need) + " bytes, got " + std::to_string(bytes));
-    *out = (uint8_t *)ws;
+// A stream that lasts as long as the context.  Any other may be destroyed
+// before the context is bound to the next, so its handle is not used then.
+static bool lasting(const har_cuda_ctx *ctx, cudaStream_t s) { return s == ctx->own_stream || s == cudaStreamLegacy; }
+
+void free_workspace(har_cuda_ctx *ctx) {
+  har_cuda_ctx::Workspace &a = ctx->ws;
+  if (a.p) {
+    if (lasting(ctx, a.stream)) cudaStreamSynchronize(a.stream);
+    else cudaEventSynchronize(a.used);
+    cudaFree(a.p);
+  }
+  if (a.used) cudaEventDestroy(a.used);
+  a = {};
+}
+
+// The workspace of one call: the caller's, or outside a capture the context's.
+// The context's is used in order by the streams that the context is bound to one
+// after the other: a call on another stream than the last use's waits for that
+// use on the device.  What it waits for is an event: recorded behind the use
+// where the stream may be gone later, and otherwise only once another stream
+// comes, so that calls on one lasting stream (torch's default one) pay nothing.
+class CallWorkspace {
+ public:
+  uint8_t *p = nullptr;
+
+  explicit CallWorkspace(har_cuda_ctx *ctx) : ctx_(ctx) {}
+  ~CallWorkspace() {
+    if (!shared_) return;
+    har_cuda_ctx::Workspace &a = ctx_->ws;
+    a.stream = ctx_->stream;
+    a.stream_id = id_;
+    if (!lasting(ctx_, a.stream)) cudaEventRecord(a.used, a.stream);
+  }
+  CallWorkspace(const CallWorkspace &) = delete;
+  CallWorkspace &operator=(const CallWorkspace &) = delete;
+
+  int32_t take(void *given, size_t bytes, size_t need, const char *who) {
+    if (need == 0) return HAR_CUDA_OK;
+    if (given) {
+      if (((uintptr_t)given & 15u) || bytes < need)
+        return set_error(ctx_, HAR_CUDA_ERR_ARG, std::string(who) + ": the workspace must be 16-byte aligned and hold " +
+                                                     std::to_string(need) + " bytes, got " + std::to_string(bytes));
+      p = (uint8_t *)given;
+      return HAR_CUDA_OK;
+    }
+    bool captured = false;
+    const int32_t st = capturing(ctx_, who, &captured);
+    if (st != HAR_CUDA_OK) return st;
+    if (captured)
+      return set_error(ctx_, HAR_CUDA_ERR_ARG, std::string(who) + ": a captured call needs a workspace of " +
+                                                   std::to_string(need) + " bytes from the caller");
+    har_cuda_ctx::Workspace &a = ctx_->ws;
+    cudaError_t e = cudaStreamGetId(ctx_->stream, &id_);
+    if (e == cudaSuccess && need > a.bytes) {
+      free_workspace(ctx_);
+      const size_t sz = (need + (1u << 20) - 1) & ~((size_t)(1u << 20) - 1);
+      if (cudaMalloc(&a.p, sz) != cudaSuccess) {
+        cudaGetLastError();
+        a.p = nullptr;
+        return set_error(ctx_, HAR_CUDA_ERR_OOM, std::string(who) + ": a workspace of " + std::to_string(sz) + " bytes failed");
+      }
+      a.bytes = sz;
+      a.stream = ctx_->own_stream;  // nobody uses it yet
+      a.stream_id = id_;
+      e = cudaEventCreateWithFlags(&a.used, cudaEventDisableTiming);
+      if (e != cudaSuccess) free_workspace(ctx_);
+    } else if (e == cudaSuccess && id_ != a.stream_id) {
+      if (lasting(ctx_, a.stream)) e = cudaEventRecord(a.used, a.stream);
+      if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx_->stream, a.used, 0);
+    }
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(ctx_, HAR_CUDA_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
+    }
+    p = (uint8_t *)a.p;
+    shared_ = true;
     return HAR_CUDA_OK;
   }
-  bool captured = false;
-  int32_t st = capturing(ctx, who, &captured);
-  if (st != HAR_CUDA_OK) return st;
-  if (captured)
-    return set_error(ctx, HAR_CUDA_ERR_ARG, std::string(who) + ": a captured call needs a workspace of " +
-                                                std::to_string(need) + " bytes from the caller");
-  st = ensure_scratch(ctx, need);
-  if (st == HAR_CUDA_OK) *out = (uint8_t *)ctx->scratch;
-  return st;
-}
+
+ private:
+  har_cuda_ctx *ctx_;
+  unsigned long long id_ = 0;
+  bool shared_ = false;
+};
 
 }  // namespace har
 
@@ -260,10 +322,10 @@ int32_t har_cuda_i8_linear(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, cons
   HAR_TRY(on.status(ctx));
   if (M == 1) ldx = w->K, ldy = w->N;
   if (i8_gemv_takes(M, w->N, w->K)) return launch_i8_gemv(ctx, w, x_dev, x_dtype, ldx, nullptr, M, y_dev, y_dtype, ldy);
-  uint8_t *ws;
-  HAR_TRY(take_workspace(ctx, workspace_dev, workspace_bytes, quantized_bytes(w, M), "i8_linear", &ws));
-  float *scale = (float *)ws;
-  int8_t *q = (int8_t *)ws + round16(sizeof(float) * (size_t)M);
+  CallWorkspace ws(ctx);
+  HAR_TRY(ws.take(workspace_dev, workspace_bytes, quantized_bytes(w, M), "i8_linear"));
+  float *scale = (float *)ws.p;
+  int8_t *q = (int8_t *)ws.p + round16(sizeof(float) * (size_t)M);
   const int64_t ldq = (int64_t)round16((size_t)w->K);
   HAR_TRY(launch_i8_quantize(ctx, x_dev, x_dtype, M, w->K, ldx, q, ldq, scale));
   return launch_i8_matmul(ctx, w, q, ldq, scale, M, y_dev, y_dtype, ldy);
@@ -319,9 +381,9 @@ int32_t har_cuda_i8_head_logprobs(har_cuda_ctx *ctx, const har_cuda_i8_weights *
   OnDevice on(ctx);
   HAR_TRY(on.status(ctx));
   if (T == 1) ldx = w->K;
-  uint8_t *ws;
-  HAR_TRY(take_workspace(ctx, workspace_dev, workspace_bytes, head_workspace_bytes(w, T, k), "i8_head_logprobs", &ws));
-  return launch_i8_head(ctx, w, x_dev, x_dtype, ldx, T, o, ws);
+  CallWorkspace ws(ctx);
+  HAR_TRY(ws.take(workspace_dev, workspace_bytes, head_workspace_bytes(w, T, k), "i8_head_logprobs"));
+  return launch_i8_head(ctx, w, x_dev, x_dtype, ldx, T, o, ws.p);
 }
 
 }  // extern "C"

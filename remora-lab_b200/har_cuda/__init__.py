@@ -504,7 +504,8 @@ class Context:
     def i8_linear(self, w: "I8Weights", x, y, workspace=None):
         """y [M][N] = x w^T through 8 bits: x [M][K] quantised per row, then
         i8_matmul.  workspace: a device tensor of w.linear_workspace(M) bytes,
-        needed only while a CUDA graph is captured; else the context's arena."""
+        needed while a CUDA graph is captured, and for calls that are to overlap
+        on two streams; else the context's own, used in order."""
         M, K, xp, ldx = _matrix(x, self.device, "i8_linear: x")
         My, N, yp, ldy = _matrix(y, self.device, "i8_linear: y")
         if K != w.K or N != w.N or My != M:

@@ -1,5 +1,6 @@
 """8-bit integer products with scales per token and channel against their
 definition in 64 bits, bit for bit: every rounding is part of the definition."""
+import ctypes as C
 import math
 
 import pytest
@@ -457,3 +458,52 @@ def test_new_weights_are_ready_for_any_stream(ctx, dtype):
     for out in y:
         assert torch.equal(out.cpu(), ref[:out.shape[0]]), out.shape
     other.close()
+
+
+def test_one_context_on_two_streams_in_turn(ctx):
+    """Calls without a workspace on two streams that nobody orders, through one
+    context: the second waits for the first's quantised rows to be done with,
+    also where the workspace grows between two calls."""
+    N, K = 3000, 1024
+    w, wq, ws = weights(ctx, 94, N, K)
+    c = har_cuda.Context(0)                          # its workspace starts empty
+    sizes = (40, 900, 333, 2000, 1500, 64, 2600, 2600)
+    xs = [rows(95 + i, m, K, ("f32", "bf16")[i % 2]) for i, m in enumerate(sizes)]
+    ys = [torch.zeros(m, N, device="cuda") for m in sizes]
+    streams = [torch.cuda.Stream(), torch.cuda.default_stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for i, (x, y) in enumerate(zip(xs, ys)):
+            with torch.cuda.stream(streams[(i + turn) % 3]):
+                c.bind_torch_stream()
+                c.i8_linear(w, x, y)
+    torch.cuda.synchronize()
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        at = sorted({0, 1, sizes[i] // 2, sizes[i] - 1})
+        assert torch.equal(y[at].cpu(), product(*quantize64(x[at]), wq, ws, torch.float32)), i
+    c.close()
+
+
+def test_stream_destroyed_before_the_next_is_bound(ctx):
+    """A stream of the caller's that is gone when the context is bound to the
+    next one: its handle is not used any more."""
+    N, K, M = 500, 256, 70
+    w, wq, ws = weights(ctx, 97, N, K)
+    runtime = torch.cuda.cudart()
+    y = [torch.zeros(M, N, device="cuda") for _ in range(4)]
+    x = [rows(98 + i, M, K) for i in range(4)]
+    torch.cuda.synchronize()
+    try:
+        for i in range(4):
+            h = C.c_void_p()
+            assert int(runtime.cudaStreamCreate(C.addressof(h))) == 0
+            ctx.check(ctx.lib.har_cuda_ctx_set_stream(ctx.handle, h))
+            ctx.i8_linear(w, x[i], y[i])
+            ctx.synchronize()
+            assert int(runtime.cudaStreamDestroy(h.value)) == 0
+    finally:
+        ctx.bind_torch_stream()
+    ctx.i8_linear(w, x[0], y[0])
+    torch.cuda.synchronize()
+    for a, b in zip(x, y):
+        assert torch.equal(b.cpu(), product(*quantize64(a), wq, ws, torch.float32))

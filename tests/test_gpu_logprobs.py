@@ -596,3 +596,27 @@ def test_large_head_with_few_tokens_in_the_last_warps(ctx, T, k):
     tok = given(42, T, V, 1)
     rows = sorted({0, 127, 128, T // 2, 160, T - 3, T - 2, T - 1} & set(range(T)))
     check_large_head(ctx, w, q, s, x, tok, k, rows=rows, what=(T, k))
+
+
+def test_head_of_one_context_on_two_streams_in_turn(ctx):
+    """Head calls without a workspace, logits stored and not, on two streams that
+    nobody orders, through one context: each has the workspace to itself."""
+    V, K, k = 240_001, 64, 6
+    w, q, s = head_of(ctx, 51, V, K)
+    c = har_cuda.Context(0)
+    sizes = (130, 20, 257, 64, 200, 300)
+    xs = [torch.randn(T, K, generator=torch.Generator().manual_seed(T)).cuda() for T in sizes]
+    toks = [given(T, T, V, 1) for T in sizes]
+    assert {unstored(T, V, k) for T in sizes} == {True, False}
+    outs = [outputs(T, 1, k) for T in sizes]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for i, o in enumerate(outs):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                c.bind_torch_stream()
+                c.i8_head_logprobs(w, xs[i], toks[i], o["logprobs"], o["entropy"], o["ids"], o["top"])
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        check_rows(o, q, s, xs[i], toks[i], k, [0, sizes[i] // 2, sizes[i] - 1], i)
+    c.close()
