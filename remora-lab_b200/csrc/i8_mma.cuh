@@ -222,7 +222,9 @@ inline int ring_stages(int bn) {
   return n < G_MAX_STAGES ? n : G_MAX_STAGES;
 }
 
-// Launch of a kernel whose blocks work in clusters of `cluster`.
+// Launch of a kernel whose blocks work in clusters of `cluster`.  `smem` is the
+// same for every launch of a kernel: its limit, set here, is the process's, and
+// threads with contexts of their own launch at the same time.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_clusters(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
                             unsigned cluster, Args... args) {

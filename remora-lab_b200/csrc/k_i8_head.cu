@@ -23,6 +23,9 @@ constexpr int H_SLOT = 2 * G_A * G_KS;    // bytes of a k-step
 // 2,048 with 5: 384 us with 40 entries and 405 with 60; with 20: 445 and 449, 24:
 // 500 and 466, 32: 3,148 and 604): a list of 60 beside three slots.
 constexpr int H_SLOTS = 4, H_CAP = 40, H_SLOTS_LONG = 3, H_CAP_LONG = 60, H_LONG = 22;
+// Bytes of either division.  Every launch asks for the larger: the function's
+// limit belongs to the process, and another thread's smaller one would refuse it.
+constexpr size_t H_SMEM = (size_t)std::max(H_SLOTS * H_SLOT + H_CAP * H_ROW, H_SLOTS_LONG * H_SLOT + H_CAP_LONG * H_ROW) + 1024;
 constexpr int H_PEERS = 16;  // parts that a part asks
 constexpr int H_JOIN = 64, H_JOIN_MOST = 320;  // threads of a joining block: one a part
 constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
@@ -645,9 +648,8 @@ int32_t launch_i8_head(har_cuda_ctx *ctx, const har_cuda_i8_weights *w, const vo
     if (st != HAR_CUDA_OK) return st;
     if (k > 0 && cudaMemsetAsync(p.best2, 0, sizeof(uint64_t) * (size_t)h.parts() * (size_t)h.Tp, ctx->stream) != cudaSuccess)
       return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_logprobs: ") + cudaGetErrorString(cudaGetLastError()));
-    const size_t smem = (size_t)p.sh.stages * H_SLOT + (size_t)cap * H_ROW + 1024;
     prof_begin(ctx);
-    const cudaError_t e = launch_clusters(i8_head_kernel, (unsigned)h.blocks(), G_THREADS, smem, ctx->stream, 2, map_x, w->map, p);
+    const cudaError_t e = launch_clusters(i8_head_kernel, (unsigned)h.blocks(), G_THREADS, H_SMEM, ctx->stream, 2, map_x, w->map, p);
     st = check_launch(ctx, "i8_head_kernel");
     if (e != cudaSuccess)
       return set_error(ctx, HAR_CUDA_ERR_CUDA, std::string("i8_head_kernel: ") + cudaGetErrorString(e));

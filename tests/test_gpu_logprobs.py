@@ -1,6 +1,7 @@
 """Log probabilities of given tokens, entropy and top alternatives against the
 definition in 64 bits, from logits and straight from hidden states."""
 import math
+import threading
 
 import pytest
 import torch
@@ -620,3 +621,42 @@ def test_head_of_one_context_on_two_streams_in_turn(ctx):
     for i, o in enumerate(outs):
         check_rows(o, q, s, xs[i], toks[i], k, [0, sizes[i] // 2, sizes[i] - 1], i)
     c.close()
+
+
+def test_two_threads_with_few_and_many_alternatives():
+    """A context and a stream a thread, one asking for 5 alternatives and one for
+    24: how much shared memory the one's lists take is no matter to the other."""
+    V, K, T, calls = 1_200_001, 16, 65, 1500
+    errors = []
+
+    def work(k):
+        try:
+            c = har_cuda.Context(0, use_torch_stream=False)
+            w = c.wrap_i8(q, s)
+            o = outputs(T, 1, k)
+            space = torch.empty(w.head_workspace(T, 1, k), dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            start.wait(60)
+            for _ in range(calls):
+                c.i8_head_logprobs(w, x, tok, o["logprobs"], o["entropy"], o["ids"], o["top"], workspace=space)
+            c.synchronize()
+            results[k] = o
+            c.close()
+        except Exception as e:
+            errors.append((k, e))
+
+    assert unstored(T, V, 5) and unstored(T, V, 24)
+    q = torch.randint(-127, 128, (V, K), dtype=torch.int8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(61))
+    s = torch.full((V,), 0.01, device="cuda")
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(62)).cuda()
+    tok = given(63, T, V, 1)
+    results, start = {}, threading.Barrier(2)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in (5, 24)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k, o in results.items():
+        check_rows(o, q, s, x, tok, k, [0, T - 1], k)
