@@ -303,7 +303,10 @@ class Context:
             raise HarCudaError(st, f"ctx_create(device={device}) failed")
         self.handle = h
         self.device = device
-        _Types.load()
+        try:
+            _Types.load()
+        except ImportError:  # calls on numpy arrays alone do without torch
+            pass
         if use_torch_stream:
             self.bind_torch_stream()
 

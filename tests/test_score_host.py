@@ -1,6 +1,9 @@
 """Refusals of the 8-bit products and log-probability calls that need no GPU:
 null contexts and handles, tensors on the CPU."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -104,3 +107,21 @@ def test_score_refuses():
             m.score([(np.zeros(5, np.float32), bad)])
     with pytest.raises(har_cuda.HarCudaError):
         m.score([(np.zeros(5, np.float32), [1])], top=33)
+
+
+def test_context_without_torch():
+    """A program that works on numpy alone makes its context without torch."""
+    code = """
+import sys
+sys.modules["torch"] = None                      # `import torch` raises ImportError
+import har_cuda
+class Library:
+    def har_cuda_ctx_create(self, device, out): return 0
+    def har_cuda_ctx_destroy(self, handle): return 0
+har_cuda.load_library = Library
+c = har_cuda.Context(0, use_torch_stream=False)
+c.close()
+"""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "remora-lab_b200")
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
