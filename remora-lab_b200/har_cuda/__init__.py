@@ -1350,10 +1350,15 @@ class CudaMoeServingModel:
         self.ctx.synchronize()
         nxt, lg = x.cpu().numpy(), logits.cpu().numpy()
         self.last_routes = [(i.cpu().numpy(), w.cpu().numpy()) for i, w in routes]
-        self.telemetry["positions"] += len(inputs)
-        self.telemetry["expert_reads"] += sum(len(np.unique(i)) for i, _ in self.last_routes)
-        self.telemetry["shared_reads"] += len(self.layers)
+        self._count_step(len(inputs), [i for i, _ in self.last_routes])
         return [StepOutcome(nxt[i], lg[i]) for i in range(len(inputs))]
+
+    def _count_step(self, positions: int, ids):
+        """One step of the layers, ids [B][k] the routes of each: its positions, the
+        experts that it read, the shared experts."""
+        self.telemetry["positions"] += positions
+        self.telemetry["expert_reads"] += sum(len(np.unique(i)) for i in ids)
+        self.telemetry["shared_reads"] += len(ids)
 
     # rows whose logits are held at a time where the head is block-quantised
     SCORE_ROWS = 128
@@ -1383,7 +1388,8 @@ class CudaMoeServingModel:
         (a row's step does not depend on the others'), and the head is applied
         once, to every position of the batch (with an 8-bit head by
         i8_head_logprobs, which stores no logits of many positions).  `top`
-        alternatives a position, at most LOGPROBS_MAX_TOP."""
+        alternatives a position, at most LOGPROBS_MAX_TOP.  telemetry counts every
+        position, and the weight reads of each step of the batch."""
         torch = self._torch
         seqs = [np.asarray(t, np.int64).reshape(-1) for _, t in inputs]
         if not 0 <= top <= LOGPROBS_MAX_TOP:
@@ -1397,11 +1403,13 @@ class CudaMoeServingModel:
         at = np.cumsum([0] + [s.size for s in seqs])  # sequence i's positions start at at[i]
         rows = torch.empty((P, self.H), dtype=torch.float32, device=self._dev)
         hid = torch.from_numpy(np.stack([np.asarray(h, np.float32).reshape(self.H) for h, _ in inputs])).to(self._dev)
+        ids = []  # the routes of every step and layer
         for i in range(max(s.size for s in seqs)):
             live = [j for j, s in enumerate(seqs) if s.size > i]
             t = torch.from_numpy(np.asarray([seqs[j][i] for j in live])).to(self._dev)
             prev = hid[live] if i == 0 else rows[torch.from_numpy(at[live] + i - 1).to(self._dev)]
-            y, _ = self._layers_device((prev + self.embed[t]).contiguous())
+            y, routes = self._layers_device((prev + self.embed[t]).contiguous())
+            ids.append([r for r, _ in routes])
             rows[torch.from_numpy(at[live] + i).to(self._dev)] = y
         nxt = np.full(P, -1, np.int32)
         for j, s in enumerate(seqs):
@@ -1409,6 +1417,13 @@ class CudaMoeServingModel:
         lp, en, ti, tl = self._score_device(rows, torch.from_numpy(nxt).to(self._dev), top)
         self.ctx.synchronize()
         lp, en, ti, tl = (v.cpu().numpy() for v in (lp, en, ti, tl))
+        if ids[0]:
+            flat = torch.cat([r for step in ids for r in step]).cpu().numpy()  # one copy
+            done = 0
+            for step in ids:
+                n = len(step) * len(step[0])
+                self._count_step(len(step[0]), np.split(flat[done:done + n], len(step)))
+                done += n
         return [ScoreOutcome(lp[a:max(a, b - 1)], en[a:b], ti[a:b], tl[a:b]) for a, b in zip(at[:-1], at[1:])]
 
     def prefill_batch(self, inputs):

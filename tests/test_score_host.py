@@ -125,3 +125,33 @@ c.close()
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "remora-lab_b200")
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+class _Routed(_Fold):
+    """Two layers of routes: a row's experts follow from how often it was folded."""
+
+    def __init__(self, V):
+        super().__init__(V)
+        self.telemetry = {"positions": 0, "expert_reads": 0, "shared_reads": 0}
+        self.step = 0
+
+    def _layers_device(self, x):
+        y, _ = super()._layers_device(x)
+        self.step += 1
+        first = torch.arange(x.shape[0], dtype=torch.int32).unsqueeze(1) % 2  # experts 0, 1 or 1, 2
+        ids = torch.cat([first, first + 1], 1)
+        return y, [(ids, None), (ids * 0 + self.step, None)]                  # the second layer: one expert a step
+
+
+def test_score_counts_what_it_folds():
+    """Positions and weight reads of scored sequences, as batch_step counts its
+    own: a step of the batch reads each expert that it uses once."""
+    m = _Routed(7)
+    h = np.zeros(7, np.float32)
+    m.score([(h, [3, 1, 6]), (h, [2]), (h, []), (h, [0, 5])], top=1)
+    assert m.batches == [3, 2, 1]
+    # first layer: rows 0 1 2 use experts {0 1 2}, rows 0 1 the same three, row 0 two
+    assert m.telemetry == {"positions": 6, "expert_reads": (3 + 1) + (3 + 1) + (2 + 1), "shared_reads": 3 * 2}
+    m.score([], top=1)
+    m.score([(h, [])])
+    assert m.telemetry["positions"] == 6
