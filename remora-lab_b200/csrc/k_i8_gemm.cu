@@ -294,11 +294,15 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 }
 
 // How a product is cut up.  Blocks a tile (cg), tokens of a tile (bn), pairs
-// that share a tile (split): the cheapest by these measures.  A k-step costs a
-// block its MMAs, 2 cycles a token at 8,192 products a cycle, and 315 at the
-// least, which issuing them takes; or its bytes, 72 a cycle, of which a pair's
-// blocks share the tokens'.  A tile costs about 1,000 cycles to fill and drain,
-// a pair 2,000 more to join, and 4,000 if its sums have to meet.  Of 220 cuts of
+// that share a tile (split): the first by this order of merit.  It ranks cuts of
+// one product and does not predict times: those are up to twice its cycles and
+// more (512 x 2,048 x 2,048 takes 8.2 us for 3.4 by it, 777 x 5,003 x 1,999 19.6
+// when aligned for 8.2, 48 x 65,536 x 2,048 29 for 12.7), since it leaves out the
+// launch, the memory's bytes and the waits for L2, which are much alike from cut to cut.
+// A k-step counts for its MMAs, 2 cycles a token at 8,192 products a cycle, and 315
+// at the least, which issuing them takes; or for its bytes, 72 a cycle, of which a
+// pair's blocks share the tokens'.  A tile counts 1,000 cycles to fill and drain, a
+// pair 2,000 more to join, and 4,000 if its sums have to meet.  Of 220 cuts of
 // 31 products from 64 x 64 x 64 to 4096^3 the cut that it names is 1.5% slower
 // than the best on average: 777 x 5,008 x 1,999 takes 19.6 us as 280 lone tiles of
 // 112 tokens and 19.9 as 140 pairs' of 128, 203 x 50,024 x 1,999 44 us alone and 38

@@ -183,7 +183,8 @@ static int gemv_rows(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 
 // 2 rows 80 and 91, 4 rows 96 and 91; 4,096 x 2,048 with 4 rows 8.2 and 12.3, 8
 // rows 10.3 and 12.3; 8 rows of 65,536 x 2,048 47 and 31; 512 x 4,096 with 4 rows
 // 10.3 and 12.3, 8 rows 16.4 and 12.3; 1,024 x 16,384 with one row 18.5 and 19.5, 2
-// rows 22.6 and 19.5.
+// rows 22.6 and 19.5.  Up to 4 rows the rule does not look at N: the 4 rows of
+// 131,072 x 4,096 lose their 5 us by it.
 bool i8_gemv_takes(int64_t M, int64_t N, int64_t K) {
   return (M <= 4 || (M <= 8 && N * K <= 8 << 20)) && gemv_rows(M) * ((K + 15) / 16 * 16) <= V_MAX_SMEM;
 }

@@ -32,7 +32,7 @@ constexpr int64_t H_TOKENS = 4096;  // tokens of one launch
 constexpr int64_t H_WALK_TOKENS = 64, H_WALK_BYTES = 12 << 20;
 
 struct HeadPlan {
-  int tt, vt, g, C, passes;         // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
+  int tt, vt, g, C;                 // token tiles, vocabulary tiles, token tiles at a time, vocabulary streams
   int64_t Tp;                       // tokens rounded up to tiles
   int parts() const { return 2 * C; }
   int blocks() const { return 2 * g * C; }
@@ -534,7 +534,7 @@ static HeadPlan head_plan(int64_t T, int64_t V, int sms) {
   for (int g = std::min(h.tt, slots); g >= 1; --g) {
     const int C = std::min({h.vt, slots / g, H_JOIN_MOST / 2}), passes = (h.tt + g - 1) / g;
     const double cost = passes * ((h.vt + C - 1) / C + 0.5);
-    if (!h.g || cost < best) best = cost, h.g = g, h.C = C, h.passes = passes;
+    if (!h.g || cost < best) best = cost, h.g = g, h.C = C;
   }
   return h;
 }
@@ -579,6 +579,8 @@ static int64_t head_chunk(int64_t T) {
 // walk takes 110 to 115 us, this kernel 72, 100, 101, 106 and 135 with 0, 1, 5, 8 and
 // 20 of them; for 203 x 50,021 x 1,999 58 to 61, and 50, 67, 72 (5) and 99 (20);
 // for 768 x 131,072 x 2,048 252 (8), 254 (20) and 262 (32), and 188, 234 and 322.
+// The threshold rests on these shapes: the product, which both ways share, grows
+// with K and the lists do not, so it is off where K is much larger or smaller.
 static bool head_walks(int64_t T, int64_t V, int k) {
   return T <= H_WALK_TOKENS || T * V * (int64_t)sizeof(float) <= (k ? std::max(k, 8) : 1) * H_WALK_BYTES;
 }
