@@ -117,7 +117,6 @@ __device__ __forceinline__ void ring_close(Ring &r, int *status) {
   }
   tc::tc_fence_after();
   if (threadIdx.x < 32) {
-    __syncwarp();
     if (CG == 2) tc::tmem_dealloc_pair(r.tmem, 512);
     else tc::tmem_dealloc(r.tmem, 512);
   }
