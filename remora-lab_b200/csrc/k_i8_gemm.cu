@@ -295,10 +295,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 
 // How a product is cut up.  Blocks a tile (cg), tokens of a tile (bn), pairs
 // that share a tile (split): the first by this order of merit.  It ranks cuts of
-// one product and does not predict times: those are up to twice its cycles and
-// more (512 x 2,048 x 2,048 takes 8.2 us for 3.4 by it, 777 x 5,003 x 1,999 19.6
-// when aligned for 8.2, 48 x 65,536 x 2,048 29 for 12.7), since it leaves out the
-// launch, the memory's bytes and the waits for L2, which are much alike from cut to cut.
+// one product and does not predict times, which are more than twice its cycles
+// (512 x 2,048 x 2,048 takes 8.2 us for 3.4 by it, 777 x 5,003 x 1,999 19.6 when
+// aligned for 8.2, 48 x 65,536 x 2,048 29 for 12.7): it leaves out the launch, the
+// memory's bytes and the waits for L2.
 // A k-step counts for its MMAs, 2 cycles a token at 8,192 products a cycle, and 315
 // at the least, which issuing them takes; or for its bytes, 72 a cycle, of which a
 // pair's blocks share the tokens'.  A tile counts 1,000 cycles to fill and drain, a
